@@ -9,6 +9,13 @@ Public functions mirror src/kernels/{adaln,fp8,rope,ctx_scale,rms}.py of the ref
     ctx_scale_rowquant                            (the gain and FP8 quantisation in one pass)
     rms_silu, add_rms_silu, shuffle_rms_silu      (VAE channel RMS norm + SiLU)
 
+and, without a counterpart there:
+
+    rowquant_int8, quantize_weight_int8, int8_linear   (8-bit integer linear layers)
+    gelu_int8, gelu_int8_bwd, int8_wgrad, int8_restore (8-bit activation checkpoints)
+    sandwich_norm, sandwich_norm_int8, sandwich_norm_bwd
+                                                  (norms before and after a block)
+
 All run through the C-ABI library ``lib/libanima_flat_b200.so`` (see
 ``include/anima_flat_b200.h``); there is no CPU fallback.
 """
@@ -16,24 +23,46 @@ All run through the C-ABI library ``lib/libanima_flat_b200.so`` (see
 from .kernels.adaln import adaln, residual_adaln
 from .kernels.ctx_scale import ctx_scale, ctx_scale_rowquant
 from .kernels.fp8 import FP8, FP8_MAX, adaln_fp8, residual_adaln_fp8, rowquant
+from .kernels.int8 import (
+    Int8Weight,
+    gelu_int8,
+    gelu_int8_bwd,
+    int8_linear,
+    int8_restore,
+    int8_wgrad,
+    quantize_weight_int8,
+    rowquant_int8,
+)
 from .kernels.rms import add_rms_silu, rms_silu, shuffle_rms_silu
 from .kernels.rope import head_norm, qkv_norm_rope
+from .kernels.sandwich import sandwich_norm, sandwich_norm_bwd, sandwich_norm_int8
 from .tables import rope_tables
 
 __all__ = [
     "FP8",
     "FP8_MAX",
+    "Int8Weight",
     "adaln",
-    "add_rms_silu",
     "adaln_fp8",
+    "add_rms_silu",
     "ctx_scale",
     "ctx_scale_rowquant",
+    "gelu_int8",
+    "gelu_int8_bwd",
     "head_norm",
+    "int8_linear",
+    "int8_restore",
+    "int8_wgrad",
     "qkv_norm_rope",
+    "quantize_weight_int8",
     "residual_adaln",
     "residual_adaln_fp8",
     "rms_silu",
     "rope_tables",
     "rowquant",
+    "rowquant_int8",
+    "sandwich_norm",
+    "sandwich_norm_bwd",
+    "sandwich_norm_int8",
     "shuffle_rms_silu",
 ]

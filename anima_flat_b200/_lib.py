@@ -45,6 +45,16 @@ SIGNATURES: dict[str, tuple] = {
     "afb_ctx_scale_bwd": (_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P),
     "afb_rms_silu": (_P, _P, _P, _P, _P, _I, _I, _I, _I, c_int, _P),
     "afb_rms_silu_bwd": (_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, c_int, _P, ctypes.c_size_t, _P),
+    "afb_rowquant_int8": (_P, _P, _P, _P, _I, _I, c_int, _P),
+    "afb_gelu_int8": (_P, _P, _P, _P, _P, _I, _I, c_int, _P),
+    "afb_gelu_int8_bwd": (_P, _P, _P, _P, _I, _I, c_int, _P),
+    "afb_int8_restore": (_P, _P, _P, _I, _I, c_int, _P),
+    "afb_int8_linear": (_P, _P, _P, _P, _P, _P, _I, _I, _I, c_int, _P),
+    "afb_int8_wgrad": (_P, _P, _P, _P, _I, _I, _I, c_int, _P),
+    "afb_sandwich_norm": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F, c_int, _P),
+    "afb_sandwich_norm_int8": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F, c_int, _P),
+    "afb_sandwich_norm_bwd": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I,
+                              _F, _F, c_int, _P, ctypes.c_size_t, _P),
 }
 
 # Workspace-size queries: name -> argument types (return size_t).
@@ -54,6 +64,7 @@ WORKSPACE_QUERIES: dict[str, tuple] = {
     "afb_qkv_norm_rope_bwd_workspace": (_I, _I, _I, _I),
     "afb_head_norm_bwd_workspace": (_I, _I, _I, _I),
     "afb_rms_silu_bwd_workspace": (_I, _I),
+    "afb_sandwich_norm_bwd_workspace": (_I, _I, _I),
 }
 
 _lib: ctypes.CDLL | None = None

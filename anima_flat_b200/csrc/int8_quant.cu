@@ -1,0 +1,301 @@
+// Row quantisation to 8-bit integers, the GELU whose input is kept in 8 bits
+// for the backward pass, and the restoring of codes.
+//
+// Per row of K elements, with a = max(max|y|, 1e-30) (afb::RowScale):
+//   s = a / 127,  q = rint(127 y / a)
+// where y is the input, the input times a vector over its columns (the
+// gradient entering a product with scaled weight rows), or GELU(input).
+//
+// Memory bound: 3 bytes an element (4 for GELU, which writes both its own
+// codes and those of its input).  A row lives in the registers of a group of
+// GROUP warps from its only read to the write of its codes; 16 elements a
+// thread and step make each access 16 bytes wide.
+#include "int8_common.cuh"
+
+namespace afb {
+
+struct QuantArgs {
+  const uint16_t* x;  // [rows, K]
+  const float* cols;  // [K] or null: factors of the columns
+  int8_t* q;          // [rows, K]: codes of x, x * cols or GELU(x)
+  float* s;           // [rows]
+  int8_t* c;          // GELU only: codes of x
+  float* cs;          // GELU only
+  int64_t rows;
+  int K;
+};
+
+enum QuantMode { kPlain = 0, kCols = 1, kGelu = 2 };
+
+__host__ __device__ constexpr int quant_block_warps(int group) { return group > 4 ? group : 4; }
+
+template <int CPL, int GROUP, int DT, int MODE>
+__global__ void __launch_bounds__(quant_block_warps(GROUP) * 32)
+rowquant_int8_kernel(const QuantArgs a) {
+  constexpr int BW = quant_block_warps(GROUP);
+  __shared__ uint32_t red[2][BW];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const int t = (warp % GROUP) * 32 + lane;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (BW / GROUP) + warp / GROUP;
+  const bool row_ok = row < a.rows;
+  const int K = a.K;
+  const int64_t base = (row_ok ? row : 0) * K;
+
+  uint4 xv[CPL][2];
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) {
+    const int e = (t + 32 * GROUP * c) * 16;
+    const bool ok = row_ok && e < K;
+    xv[c][0] = ok ? ld_stream(a.x + base + e) : make_uint4(0, 0, 0, 0);
+    xv[c][1] = ok ? ld_stream(a.x + base + e + 8) : make_uint4(0, 0, 0, 0);
+  }
+  f2_t y[CPL][2][4];
+  uint32_t top[2] = {0, 0};  // of y; of x where GELU keeps both
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) {
+    const int e = (t + 32 * GROUP * c) * 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float f[8];
+      if (MODE == kCols) {
+        const bool ok = row_ok && e < K;
+        const float4 lo = ok ? ld_keep_f4(a.cols + e + 8 * h) : make_float4(0, 0, 0, 0);
+        const float4 hi = ok ? ld_keep_f4(a.cols + e + 8 * h + 4) : make_float4(0, 0, 0, 0);
+        f[0] = lo.x; f[1] = lo.y; f[2] = lo.z; f[3] = lo.w;
+        f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f2_t v = unpack2<DT>(word(xv[c][h], j));
+        if (MODE == kGelu) top[1] = max_bits2(top[1], v);
+        y[c][h][j] = MODE == kGelu ? fast_gelu2(v) : MODE == kCols ? mul2(v, f2(f[2 * j], f[2 * j + 1])) : v;
+        top[0] = max_bits2(top[0], y[c][h][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < (MODE == kGelu ? 2 : 1); ++n) top[n] = warp_max_u32(top[n]);
+  if (GROUP > 1) {
+    if (lane == 0) {
+      red[0][warp] = top[0];
+      if (MODE == kGelu) red[1][warp] = top[1];
+    }
+    __syncthreads();
+    const int w0 = (warp / GROUP) * GROUP;
+#pragma unroll
+    for (int w = 0; w < GROUP; ++w) {
+      top[0] = max(top[0], red[0][w0 + w]);
+      if (MODE == kGelu) top[1] = max(top[1], red[1][w0 + w]);
+    }
+  }
+  if (!row_ok) return;
+  const RowScale r = row_scale(top[0]);
+  if (t == 0) a.s[row] = r.s;
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) {
+    const int e = (t + 32 * GROUP * c) * 16;
+    if (e >= K) continue;
+    const uint2 lo = codes8(y[c][0], r), hi = codes8(y[c][1], r);
+    st16(a.q + base + e, make_uint4(lo.x, lo.y, hi.x, hi.y));
+  }
+  if (MODE == kGelu) {
+    const RowScale rx = row_scale(top[1]);
+    if (t == 0) a.cs[row] = rx.s;
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      const int e = (t + 32 * GROUP * c) * 16;
+      if (e >= K) continue;
+      uint2 o[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f2_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = unpack2<DT>(word(xv[c][h], j));
+        o[h] = codes8(v, rx);
+      }
+      st16(a.c + base + e, make_uint4(o[0].x, o[0].y, o[1].x, o[1].y));
+    }
+  }
+}
+
+// The smallest power-of-two group whose threads hold at most two chunks of 16.
+static bool quant_shape(int64_t K, int* group, int* cpl) {
+  const int64_t chunks = K / 16;
+  int g = 1;
+  while (g < 16 && chunks > 64 * g) g <<= 1;
+  *group = g;
+  *cpl = chunks > 32 * g ? 2 : 1;
+  return K >= 16 && K % 16 == 0 && chunks <= 64 * g;
+}
+
+template <int GROUP, int DT, int MODE>
+static cudaError_t launch_quant_g(const QuantArgs& a, int cpl, cudaStream_t st) {
+  constexpr int BW = quant_block_warps(GROUP);
+  const int64_t per = BW / GROUP;
+  const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per)), block(BW * 32);
+  return cpl == 1 ? launch_pdl(rowquant_int8_kernel<1, GROUP, DT, MODE>, grid, block, 0, st, a)
+                  : launch_pdl(rowquant_int8_kernel<2, GROUP, DT, MODE>, grid, block, 0, st, a);
+}
+
+template <int DT, int MODE>
+static cudaError_t launch_quant(const QuantArgs& a, cudaStream_t st) {
+  int group = 0, cpl = 0;
+  if (!quant_shape(a.K, &group, &cpl)) return cudaErrorInvalidValue;
+  switch (group) {
+    case 1: return launch_quant_g<1, DT, MODE>(a, cpl, st);
+    case 2: return launch_quant_g<2, DT, MODE>(a, cpl, st);
+    case 4: return launch_quant_g<4, DT, MODE>(a, cpl, st);
+    case 8: return launch_quant_g<8, DT, MODE>(a, cpl, st);
+    default: return launch_quant_g<16, DT, MODE>(a, cpl, st);
+  }
+}
+
+// ------------------------------------------------------------ restore, GELU' --
+struct RestoreArgs {
+  const int8_t* q;     // [rows, K]
+  const float* s;      // [rows]
+  const uint16_t* dy;  // GELU' only: [rows, K]
+  uint16_t* y;         // [rows, K]
+  int64_t chunks;      // rows * K / 16
+  DivU32 per_row;      // K / 16
+};
+
+// d/dv of v * Phi(v) = Phi(v) + v phi(v), with erf by Abramowitz & Stegun
+// 7.1.26 (|error| <= 1.5e-7): for a = |v| / sqrt 2, t = 1 / (1 + p a),
+// 1 - erf(a) = poly(t) exp(-a^2), and phi(v) holds the same exponential.
+__device__ __forceinline__ float gelu_slope(float v) {
+  const float a = fabsf(v);
+  float t, e;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(__fmaf_rn(a, 0.3275911f * 0.707106769084930419921875f, 1.0f)));
+  float p = __fmaf_rn(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  p = __fmaf_rn(p, t, 0.5f * 1.421413741f);
+  p = __fmaf_rn(p, t, 0.5f * -0.284496736f);
+  p = __fmaf_rn(p, t, 0.5f * 0.254829592f);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v * v) * -0.721347520444481703680f));
+  const float tail = p * t * e;  // 1 - Phi(|v|)
+  const float cdf = v < 0.0f ? tail : 1.0f - tail;
+  return __fmaf_rn(v * 0.3989422804014327f, e, cdf);
+}
+
+template <int DT, bool SLOPE>
+__global__ void __launch_bounds__(256) restore_kernel(const RestoreArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= a.chunks) return;
+  const uint4 qv = ld_stream(a.q + i * 16);
+  uint4 g[2] = {};
+  if (SLOPE) {
+    g[0] = ld_stream(a.dy + i * 16);
+    g[1] = ld_stream(a.dy + i * 16 + 8);
+  }
+  const float s = __ldg(a.s + div_u32(a.per_row, i));
+  uint4 o[2];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const f2_t v = mul2(code_pair(word(qv, k >> 1), k & 1), splat2(s));
+    uint32_t& w = word_ref(o[k >> 2], k & 3);
+    if (SLOPE) {
+      const f2_t d = unpack2<DT>(word(g[k >> 2], k & 3));
+      w = pack2<DT>(f2lo(d) * gelu_slope(f2lo(v)), f2hi(d) * gelu_slope(f2hi(v)));
+    } else {
+      w = pack2<DT>(v);
+    }
+  }
+  st16(a.y + i * 16, o[0]);
+  st16(a.y + i * 16 + 8, o[1]);
+}
+
+template <bool SLOPE>
+static cudaError_t launch_restore(const RestoreArgs& a, int dtype, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>((a.chunks + 255) / 256));
+  return dtype == kBf16 ? launch_pdl(restore_kernel<kBf16, SLOPE>, grid, dim3(256), 0, st, a)
+                        : launch_pdl(restore_kernel<kFp16, SLOPE>, grid, dim3(256), 0, st, a);
+}
+
+// rows * K / 16 chunks of 256-thread blocks must fit the grid's x extent.
+static bool check_quant(int64_t rows, int64_t K, int dtype) {
+  int group = 0, cpl = 0;
+  return check(rows >= 0 && rows <= INT64_C(0x7fffffff), "rows must be in [0, 2^31)") &&
+         check(quant_shape(K, &group, &cpl),
+               "K must be a multiple of 16 in [16, 16384], got " + std::to_string(K)) &&
+         check_dtype(dtype);
+}
+
+}  // namespace afb
+
+using namespace afb;
+
+extern "C" int afb_rowquant_int8(const void* x, const void* cols, void* q, void* s, int64_t rows, int64_t K,
+                                 int dtype, void* stream) {
+  ApiGuard g("afb_rowquant_int8");
+  if (!check_quant(rows, K, dtype)) return g.fail();
+  if (rows == 0) return 0;
+  if (!check_ptrs({x, q}, {"x", "q"}) || !check_ptr4(s, "s") ||
+      !check(cols == nullptr || aligned(cols, 16), "cols is not 16-byte aligned"))
+    return g.fail();
+  QuantArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.cols = static_cast<const float*>(cols);
+  a.q = static_cast<int8_t*>(q);
+  a.s = static_cast<float*>(s);
+  a.rows = rows;
+  a.K = static_cast<int>(K);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (cols != nullptr)
+    return g.done(dtype == kBf16 ? launch_quant<kBf16, kCols>(a, st) : launch_quant<kFp16, kCols>(a, st));
+  return g.done(dtype == kBf16 ? launch_quant<kBf16, kPlain>(a, st) : launch_quant<kFp16, kPlain>(a, st));
+}
+
+extern "C" int afb_gelu_int8(const void* x, void* q, void* s, void* c, void* cs, int64_t rows, int64_t K,
+                             int dtype, void* stream) {
+  ApiGuard g("afb_gelu_int8");
+  if (!check_quant(rows, K, dtype)) return g.fail();
+  if (rows == 0) return 0;
+  if (!check_ptrs({x, q, c}, {"x", "q", "c"}) || !check_ptr4(s, "s") || !check_ptr4(cs, "cs")) return g.fail();
+  QuantArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.q = static_cast<int8_t*>(q);
+  a.s = static_cast<float*>(s);
+  a.c = static_cast<int8_t*>(c);
+  a.cs = static_cast<float*>(cs);
+  a.rows = rows;
+  a.K = static_cast<int>(K);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return g.done(dtype == kBf16 ? launch_quant<kBf16, kGelu>(a, st) : launch_quant<kFp16, kGelu>(a, st));
+}
+
+static int restore(const char* name, const void* dy, const void* q, const void* s, void* y, int64_t rows, int64_t K,
+                   int dtype, void* stream) {
+  ApiGuard g(name);
+  if (!check_quant(rows, K, dtype)) return g.fail();
+  if (rows == 0) return 0;
+  if (!check_ptrs({q, y}, {"q", "y"}) || !check_ptr4(s, "s") ||
+      !check(dy == nullptr || aligned(dy, 16), "dy is not 16-byte aligned"))
+    return g.fail();
+  RestoreArgs a{};
+  a.q = static_cast<const int8_t*>(q);
+  a.s = static_cast<const float*>(s);
+  a.dy = static_cast<const uint16_t*>(dy);
+  a.y = static_cast<uint16_t*>(y);
+  a.chunks = rows * (K / 16);
+  a.per_row = make_divu32(K / 16);
+  if (!check((a.chunks + 255) / 256 <= INT64_C(0x7fffffff), "rows * K is too large")) return g.fail();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return g.done(dy != nullptr ? launch_restore<true>(a, dtype, st) : launch_restore<false>(a, dtype, st));
+}
+
+extern "C" int afb_int8_restore(const void* q, const void* s, void* y, int64_t rows, int64_t K, int dtype,
+                                void* stream) {
+  return restore("afb_int8_restore", nullptr, q, s, y, rows, K, dtype, stream);
+}
+
+extern "C" int afb_gelu_int8_bwd(const void* dy, const void* c, const void* cs, void* dx, int64_t rows, int64_t K,
+                                 int dtype, void* stream) {
+  ApiGuard g("afb_gelu_int8_bwd");
+  if (rows != 0 && !check(dy != nullptr, "dy is null")) return g.fail();
+  return restore("afb_gelu_int8_bwd", dy, c, cs, dx, rows, K, dtype, stream);
+}

@@ -34,3 +34,31 @@ def _check_vec(t: torch.Tensor, batch: int, dim: int, name: str) -> None:
 def _stream(t: torch.Tensor) -> int:
     """Handle of the current CUDA stream on the tensor's device."""
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+# dtype codes of the C ABI's entry points that take both 16-bit types.
+HALF_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _check_half(what: str, t: torch.Tensor) -> None:
+    if t.dtype not in HALF_TYPES:
+        raise ValueError(f"{what} must be torch.bfloat16 or torch.float16, got {t.dtype}")
+
+
+def _check_same_device(*ts: torch.Tensor | None) -> None:
+    """Raise ValueError unless all tensors are on one CUDA device."""
+    device = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("CUDA tensors required")
+        if device is not None and t.device != device:
+            raise ValueError(f"tensors are on {device} and {t.device}")
+        device = t.device
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and 16-byte aligned: a copy only where `t` is neither."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()

@@ -267,6 +267,75 @@ int afb_rms_silu_bwd(const void* s, const void* gamma, const void* dy, const voi
                      void* dgamma, int64_t rows, int64_t H, int64_t W, int64_t channels,
                      int shuffled, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ----------------------------------------------------------------------- */
+/* 8-bit integer linear and 8-bit checkpoints (no reference counterpart)    */
+/* ----------------------------------------------------------------------- */
+/* dtype: type of the activations, 0 bf16 or 1 fp16.  Codes are int8; a row of
+ * codes has one fp32 scale: with a = max(max|y|, 1e-30) over the row,
+ * s = a / 127 and q = rint(127 y / a), half to even.  A row that holds an
+ * infinity or a NaN gets that as its scale and zero codes.  K a multiple of
+ * 16, at most 16384 unless said otherwise; rows = 0 does nothing. */
+
+/* Codes of x [rows, K], or of x * cols where cols [K] fp32 is not NULL (the
+ * gradient that enters a product with scaled weight rows). */
+int afb_rowquant_int8(const void* x, const void* cols, void* q, void* s, int64_t rows, int64_t K,
+                      int dtype, void* stream);
+
+/* q, s: codes of GELU(x) (erf form, A&S 7.1.26); c, cs: codes of x, the
+ * checkpoint that afb_gelu_int8_bwd reads. */
+int afb_gelu_int8(const void* x, void* q, void* s, void* c, void* cs, int64_t rows, int64_t K,
+                  int dtype, void* stream);
+
+/* dx = dy * GELU'(c * cs); dy, dx [rows, K]. */
+int afb_gelu_int8_bwd(const void* dy, const void* c, const void* cs, void* dx, int64_t rows,
+                      int64_t K, int dtype, void* stream);
+
+/* y = q * s, [rows, K] of `dtype`. */
+int afb_int8_restore(const void* q, const void* s, void* y, int64_t rows, int64_t K, int dtype,
+                     void* stream);
+
+/* y[m, n] = (sum_k q[m, k] w[n, k]) * s[m] * v[n] + bias[n], the sum exact in
+ * 32-bit integers.  q [M, K], w [N, K] int8; s [M], v [N] fp32; bias [N] of
+ * `dtype` or NULL; y [M, N].  K at most 131072, N any. */
+int afb_int8_linear(const void* q, const void* s, const void* w, const void* v, const void* bias,
+                    void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream);
+
+/* dw[n, k] = sum_t dy[t, n] q[t, k] s[t], summed in fp32.  dy [rows, N], N a
+ * multiple of 8; q [rows, K], K a multiple of 16; s [rows]; dw [N, K] of
+ * `dtype` (zero where rows = 0). */
+int afb_int8_wgrad(const void* dy, const void* q, const void* s, void* dw, int64_t rows, int64_t N,
+                   int64_t K, int dtype, void* stream);
+
+/* ----------------------------------------------------------------------- */
+/* Norms before and after a block (no reference counterpart)                */
+/* ----------------------------------------------------------------------- */
+/* With rms(v) = v / sqrt(mean(v^2) + eps) over a row:
+ *   z = residual_scale * residual + gate * (rms(x) * post_weight)
+ *   h = rms(z) * pre_weight * scale + shift        (z as stored)
+ * x, residual, h, z [batch, seq, dim] of `dtype` (0 bf16, 1 fp16); gate,
+ * shift, scale [batch, dim] of `dtype`, each NULL for 1, 0, 1; post_weight,
+ * pre_weight [dim] fp32.  dim a multiple of 8 up to 4096.  The _int8 form
+ * returns h as codes q [batch * seq, dim] with scales s [batch * seq]. */
+int afb_sandwich_norm(const void* x, const void* residual, const void* gate,
+                      const void* post_weight, const void* pre_weight, const void* shift,
+                      const void* scale, void* h, void* z, int64_t batch, int64_t seq, int64_t dim,
+                      float residual_scale, float eps, int dtype, void* stream);
+int afb_sandwich_norm_int8(const void* x, const void* residual, const void* gate,
+                           const void* post_weight, const void* pre_weight, const void* shift,
+                           const void* scale, void* q, void* s, void* z, int64_t batch, int64_t seq,
+                           int64_t dim, float residual_scale, float eps, int dtype, void* stream);
+
+/* Gradients: dx, dres [batch, seq, dim]; dgate, dshift, dscale [batch, dim],
+ * each NULL if unwanted; dpost, dpre [dim] fp32.  gz may be NULL.  batch and
+ * seq at least 1. */
+size_t afb_sandwich_norm_bwd_workspace(int64_t batch, int64_t seq, int64_t dim);
+int afb_sandwich_norm_bwd(const void* gh, const void* gz, const void* z, const void* x,
+                          const void* gate, const void* post_weight, const void* pre_weight,
+                          const void* scale, void* dx, void* dres, void* dgate, void* dpost,
+                          void* dpre, void* dshift, void* dscale, int64_t batch, int64_t seq,
+                          int64_t dim, float residual_scale, float eps, int dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
