@@ -85,7 +85,8 @@ static int device_status(int* status, bool clear, const char* name) {
   using Reader = cudaError_t (*)(int*, bool);
   static const Reader readers[] = {afb::read_status_adaln_fwd, afb::read_status_headnorm_fwd,
                                    afb::read_status_headnorm_bwd, afb::read_status_adaln_bwd,
-                                   afb::read_status_rms, afb::read_status_probe};
+                                   afb::read_status_rms, afb::read_status_probe,
+                                   afb::read_status_int8_linear};
   int all = 0;
   for (Reader r : readers) {
     int v = 0;

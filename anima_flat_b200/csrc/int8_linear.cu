@@ -1,59 +1,302 @@
 // Matrix product in 8-bit integers with a scale per token and per channel:
 //   y[m, n] = (sum_k q[m, k] w[n, k]) * s[m] * v[n] + bias[n]
-// The sum is exact in 32-bit integers (K <= 131072: 127^2 K < 2^31).
+// The sum is exact in 32-bit integers (K <= 131072: 127^2 K < 2^31), so the
+// order of its parts does not matter.
+//
+// A tile is 128 channels by BN tokens: the weight rows are the first operand
+// of the matrix instruction (tensor-memory lanes), the tokens the second
+// (columns), so that a warp of the epilogue keeps its 32 channels' scales and
+// biases in registers.  TMA brings both in blocks of 128 bytes along k; one
+// thread issues the copies, one the matrix instructions, four warps the
+// epilogue, which for large products overlaps the next tile's main loop (two
+// accumulators in tensor memory).  Few tiles are split along k over a cluster,
+// whose parts are added through distributed shared memory.
 #include "int8_common.cuh"
+#include "tc_device.cuh"
+
+#include <algorithm>
 
 namespace afb {
 
 struct LinearArgs {
-  const int8_t* q;       // [M, K]
   const float* s;        // [M]
-  const int8_t* w;       // [N, K]
   const float* v;        // [N]
   const uint16_t* bias;  // [N] or null
   uint16_t* y;           // [M, N]
   int M, N, K;
+  int ntiles, tiles;     // tiles along N, and in all
 };
 
-// 64 x 64 outputs a block of 256 threads, 64 k a step, dp4a.
-template <int DT>
-__global__ void __launch_bounds__(256) int8_linear_kernel(const LinearArgs a) {
-  __shared__ int aq[64][17], bw[64][17];
+constexpr int kTileN = 128;    // channels of a tile
+constexpr int kKBlock = 128;   // k of a stage: one swizzled row of 128 bytes
+constexpr int kThreads = 192;  // copy, matrix, four epilogue warps
+
+__host__ __device__ constexpr int lin_stage_bytes(int bn) { return (kTileN + bn) * kKBlock; }
+__host__ __device__ constexpr int lin_stages(int bn) { return bn >= 256 ? 4 : bn >= 128 ? 6 : 8; }
+__host__ __device__ constexpr int lin_smem(int bn) { return lin_stages(bn) * lin_stage_bytes(bn) + 1024; }
+__host__ __device__ constexpr int lin_tmem(int bn) { return 2 * bn < 32 ? 32 : 2 * bn; }
+
+__device__ __forceinline__ float scaled(uint32_t acc, float s, float v, float b) {
+  return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(acc)), s), v), b);
+}
+
+template <int BN, int DT>
+__global__ void __launch_bounds__(kThreads, 1)
+int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap,
+                   const LinearArgs a, int split) {
+  constexpr int ST = lin_stages(BN), SB = lin_stage_bytes(BN);
+  extern __shared__ uint8_t dyn[];
+  __shared__ __align__(8) uint64_t bars[2 * ST + 4];
+  __shared__ __align__(8) float sm[2][BN];
+  __shared__ __align__(128) uint8_t out[4][2][1024];  // a warp's 16 tokens x 32 channels, twice
+  __shared__ uint32_t tslot;
+  const uint32_t ring = (smem_addr(dyn) + 1023) & ~1023u;
+  const uint32_t full = smem_addr(bars), empty = full + 8 * ST, accf = empty + 8 * ST, acce = accf + 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    prefetch_map(&wmap);
+    prefetch_map(&qmap);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(accf + 8 * i, 1);
+      mbar_init(acce + 8 * i, 4);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(smem_addr(&tslot), lin_tmem(BN));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tslot;
   pdl_wait();
   pdl_trigger();
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int lr = threadIdx.x >> 2, lc = (threadIdx.x & 3) * 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 64) {
-    const bool kok = k0 + lc * 4 < a.K;
-    const int4 z = make_int4(0, 0, 0, 0);
-    const int4 qa = kok && m0 + lr < a.M
-                        ? *reinterpret_cast<const int4*>(a.q + static_cast<int64_t>(m0 + lr) * a.K + k0 + lc * 4) : z;
-    const int4 wa = kok && n0 + lr < a.N
-                        ? *reinterpret_cast<const int4*>(a.w + static_cast<int64_t>(n0 + lr) * a.K + k0 + lc * 4) : z;
-    aq[lr][lc] = qa.x; aq[lr][lc + 1] = qa.y; aq[lr][lc + 2] = qa.z; aq[lr][lc + 3] = qa.w;
-    bw[lr][lc] = wa.x; bw[lr][lc + 1] = wa.y; bw[lr][lc + 2] = wa.z; bw[lr][lc + 3] = wa.w;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(aq[ty + 16 * i][k], bw[tx + 16 * j][k], acc[i][j]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m >= a.M || n >= a.N) continue;
-      float f = static_cast<float>(acc[i][j]) * __ldg(a.s + m) * __ldg(a.v + n);
-      if (a.bias != nullptr) f += load1<DT>(a.bias + n);
-      a.y[static_cast<int64_t>(m) * a.N + n] = static_cast<uint16_t>(pack2<DT>(f, 0.0f));
+
+  const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int blocks = (a.K + kKBlock - 1) / kKBlock;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(blocks) * rank / split);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / split);
+  const int first = static_cast<int>(blockIdx.x) / split, step = static_cast<int>(gridDim.x) / split;
+
+  if (warp == 0 && lane == 0) {
+    // Copies: a stage is refilled once the matrix instructions that read it
+    // are done.
+    int it = 0, sent = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < a.tiles; tile += step) {
+      const int n0 = (tile % a.ntiles) * kTileN, m0 = (tile / a.ntiles) * BN;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int st = it % ST;
+        if (it >= ST && !mbar_wait(empty + 8 * st, ((it / ST) - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(full + 8 * st, SB);
+        tma_load(ring + st * SB, &wmap, kb * kKBlock, n0, full + 8 * st);
+        tma_load(ring + st * SB + kTileN * kKBlock, &qmap, kb * kKBlock, m0, full + 8 * st);
+        sent = it + 1;
+      }
     }
+    // After a wait that gave up: the copies still in flight land before the
+    // block ends.
+    if (!ok)
+      for (int i = sent > ST ? sent - ST : 0; i < sent; ++i) mbar_wait(full + 8 * (i % ST), (i / ST) & 1);
+  } else if (warp == 1 && lane == 0) {
+    // 32-bit sums of signed bytes, BN columns, 128 lanes.
+    constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileN >> 4) << 24);
+    int it = 0, n = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < a.tiles; tile += step, ++n) {
+      const int buf = n & 1;
+      if (n >= 2 && !mbar_wait(acce + 8 * buf, ((n >> 1) - 1) & 1)) break;
+      tc_fence_after();
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int st = it % ST;
+        if (!mbar_wait(full + 8 * st, (it / ST) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t da = smem_desc(ring + st * SB, 16, 1024);
+        const uint64_t db = smem_desc(ring + st * SB + kTileN * kKBlock, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < kKBlock / 32; ++k)
+          mma_i8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, kb > kb0 || k > 0);
+        mma_commit(empty + 8 * st);
+      }
+      mma_commit(accf + 8 * buf);
+    }
+  } else if (warp >= 2) {
+    const int quad = warp & 3;  // the tensor-memory lanes that this warp may read
+    const int et = static_cast<int>(threadIdx.x) - 64;
+    const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    int n = 0;
+    bool ok = true;  // after a wait that gave up, only the barriers go on
+    for (int tile = first; tile < a.tiles; tile += step, ++n) {
+      const int buf = n & 1;
+      const int n0 = (tile % a.ntiles) * kTileN, m0 = (tile / a.ntiles) * BN;
+      const int ch = n0 + quad * 32 + lane;
+      const bool nok = ch < a.N;
+      const float vn = nok ? __ldg(a.v + ch) : 0.0f;
+      const float b = nok && a.bias != nullptr ? load1<DT>(a.bias + ch) : 0.0f;
+      for (int i = et; i < BN; i += 128) sm[buf][i] = m0 + i < a.M ? __ldg(a.s + m0 + i) : 0.0f;
+      named_bar_sync(1, 128);
+      ok = ok && mbar_wait(accf + 8 * buf, (n >> 1) & 1);
+      if (!ok) continue;
+      tc_fence_after();
+      const int cols = min(BN, a.M - m0);
+      if (split == 1) {
+        // 16 tokens at a time: fragments of 8 channels x 8 tokens, scaled and
+        // rounded, are transposed into rows of 32 channels, which leave as
+        // whole 64-byte runs.  16-byte chunks of the rows are swizzled, so
+        // that neither side meets a bank twice.
+        float vf[4], bf[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          vf[g] = __shfl_sync(kFull, vn, (lane >> 2) + 8 * g);
+          bf[g] = __shfl_sync(kFull, b, (lane >> 2) + 8 * g);
+        }
+        const uint32_t st0 = smem_addr(out[warp - 2][0]);
+        const int run = n0 + quad * 32;
+        const bool wide = a.N % 8 == 0;
+#pragma unroll 2
+        for (int c = 0; c < cols; c += 16) {
+          const uint32_t stage = st0 + ((c >> 4) & 1) * 1024;
+          uint32_t v[2][8];
+          tmem_ld_frag2(trow + buf * BN + c, v[0]);
+          tmem_ld_frag2(trow + (16u << 16) + buf * BN + c, v[1]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 s2 = *reinterpret_cast<const float2*>(&sm[buf][c + 8 * i + 2 * (lane & 3)]);
+            uint32_t o[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const uint32_t* p = &v[g >> 1][4 * i + 2 * (g & 1)];
+              o[g] = pack2<DT>(scaled(p[0], s2.x, vf[g], bf[g]), scaled(p[1], s2.y, vf[g], bf[g]));
+            }
+            const int tok = 8 * i + (lane & 7);
+            stmatrix_trans(stage + tok * 64 + (((lane >> 3) ^ (tok >> 1)) & 3) * 16, o);
+          }
+          __syncwarp();
+          if (wide) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int tok = 8 * i + (lane >> 2), at = run + (lane & 3) * 8;
+              const uint4 w = lds16a(stage + tok * 64 + (((lane & 3) ^ (tok >> 1)) & 3) * 16);
+              if (c + tok < cols && at < a.N) st16(a.y + static_cast<int64_t>(m0 + c + tok) * a.N + at, w);
+            }
+          } else {
+#pragma unroll 4
+            for (int tok = 0; tok < 16; ++tok) {
+              uint16_t w;
+              asm volatile("ld.shared.u16 %0, [%1];"
+                           : "=h"(w)
+                           : "r"(stage + tok * 64 + (((lane >> 3) ^ (tok >> 1)) & 3) * 16 + (lane & 7) * 2)
+                           : "memory");
+              if (c + tok < cols && nok) a.y[static_cast<int64_t>(m0 + c + tok) * a.N + ch] = w;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acce + 8 * buf);
+      } else {
+        // The ring is free: all its copies were read by the instructions that
+        // the accumulator waited for.  Column c, lane l at (c * 128 + l) * 4.
+        const uint32_t at = ring + (quad * 32 + lane) * 4;
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(trow + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (c + i) * 512), "r"(kb1 > kb0 ? v[i] : 0u) : "memory");
+        }
+      }
+    }
+  }
+  if (split > 1) {
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2) {
+      const int quad = warp & 3;
+      const int n0 = (first % a.ntiles) * kTileN, m0 = (first / a.ntiles) * BN;
+      const int ch = n0 + quad * 32 + lane;
+      const int cols = min(BN, a.M - m0);
+      const bool nok = ch < a.N;
+      const float vn = nok ? __ldg(a.v + ch) : 0.0f;
+      const float b = nok && a.bias != nullptr ? load1<DT>(a.bias + ch) : 0.0f;
+      const uint32_t at = ring + (quad * 32 + lane) * 4;
+      for (int c = rank; c < cols; c += split) {
+        uint32_t acc = 0;
+        for (int r = 0; r < split; ++r) acc += peer_ld(peer_addr(at + c * 512, r));
+        if (nok)
+          a.y[static_cast<int64_t>(m0 + c) * a.N + ch] = static_cast<uint16_t>(pack2<DT>(scaled(acc, sm[0][c], vn, b), 0.0f));
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_free(tmem, lin_tmem(BN));
+  }
 }
+
+template <int BN, int DT>
+static cudaError_t launch_linear(const void* q, const void* w, LinearArgs a, int split, cudaStream_t st) {
+  CUtensorMap wmap, qmap;
+  const uint64_t K = static_cast<uint64_t>(a.K);
+  cudaError_t e = make_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w, K, a.N, K, kKBlock, kTileN);
+  if (e == cudaSuccess)
+    e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, q, K, a.M, K, kKBlock, BN);
+  if (e == cudaSuccess) e = ensure_smem(int8_linear_kernel<BN, DT>, lin_smem(BN));
+  if (e != cudaSuccess) return e;
+  a.ntiles = (a.N + kTileN - 1) / kTileN;
+  a.tiles = a.ntiles * ((a.M + BN - 1) / BN);
+  const int grid = split > 1 ? a.tiles * split : std::min(a.tiles, device_info().sms);
+  return launch_cluster(int8_linear_kernel<BN, DT>, dim3(grid), dim3(kThreads), lin_smem(BN), split, st, wmap, qmap, a,
+                        split);
+}
+
+// Tokens of a tile and parts along k.  Up to 128 tokens one tile holds them
+// all; above, the widest tile that still gives every multiprocessor one.  What
+// is left idle goes to parts of at least two k blocks.
+static void linear_shape(int M, int N, int K, int sms, int* bn, int* split) {
+  const int64_t nt = (N + kTileN - 1) / kTileN;
+  auto tiles = [&](int b) { return nt * ((M + b - 1) / b); };
+  int b = 16;
+  while (b < 256 && b < M && (b < 128 || tiles(2 * b) >= sms)) b *= 2;
+  const int blocks = (K + kKBlock - 1) / kKBlock;
+  int s = 1;
+  while (s < 8 && b < 256 && tiles(b) * s * 2 <= sms && blocks / (2 * s) >= 2) s *= 2;
+  *bn = b;
+  *split = s;
+}
+
+template <int DT>
+static cudaError_t linear(const void* q, const void* w, const LinearArgs& a, cudaStream_t st) {
+  const DeviceInfo& d = device_info();
+  if (d.error != cudaSuccess) return d.error;
+  int bn, split;
+  linear_shape(a.M, a.N, a.K, d.sms, &bn, &split);
+  switch (bn) {
+    case 16: return launch_linear<16, DT>(q, w, a, split, st);
+    case 32: return launch_linear<32, DT>(q, w, a, split, st);
+    case 64: return launch_linear<64, DT>(q, w, a, split, st);
+    case 128: return launch_linear<128, DT>(q, w, a, split, st);
+    default: return launch_linear<256, DT>(q, w, a, split, st);
+  }
+}
+
+cudaError_t read_status_int8_linear(int* status, bool clear) { return tu_status(status, clear); }
 
 }  // namespace afb
 
@@ -68,15 +311,18 @@ extern "C" int afb_int8_linear(const void* q, const void* s, const void* w, cons
     return g.fail();
   if (M == 0) return 0;
   if (!check_ptrs({q, w}, {"q", "w"}) || !check_ptr4(s, "s") || !check_ptr4(v, "v") ||
-      !check(y != nullptr && aligned(y, 2), "y is null or not 2-byte aligned") ||
+      !check(y != nullptr && aligned(y, 16), "y is null or not 16-byte aligned") ||
       !check(aligned(bias, 2), "bias is not 2-byte aligned"))
     return g.fail();
-  LinearArgs a{static_cast<const int8_t*>(q), static_cast<const float*>(s), static_cast<const int8_t*>(w),
-               static_cast<const float*>(v), static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y),
-               static_cast<int>(M), static_cast<int>(N), static_cast<int>(K)};
-  const dim3 grid(static_cast<unsigned>((N + 63) / 64), static_cast<unsigned>((M + 63) / 64));
-  if (!check(grid.y <= 65535, "M is too large")) return g.fail();
+  LinearArgs a{};
+  a.s = static_cast<const float*>(s);
+  a.v = static_cast<const float*>(v);
+  a.bias = static_cast<const uint16_t*>(bias);
+  a.y = static_cast<uint16_t*>(y);
+  a.M = static_cast<int>(M);
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  if (!check(((M + 15) / 16) * ((N + kTileN - 1) / kTileN) <= (1 << 27), "M * N is too large")) return g.fail();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return g.done(dtype == kBf16 ? launch_pdl(int8_linear_kernel<kBf16>, grid, dim3(256), 0, st, a)
-                               : launch_pdl(int8_linear_kernel<kFp16>, grid, dim3(256), 0, st, a));
+  return g.done(dtype == kBf16 ? linear<kBf16>(q, w, a, st) : linear<kFp16>(q, w, a, st));
 }
