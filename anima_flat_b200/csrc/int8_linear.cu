@@ -32,7 +32,7 @@ constexpr int kKBlock = 128;   // k of a stage: one swizzled row of 128 bytes
 constexpr int kThreads = 192;  // copy, matrix, four epilogue warps
 
 __host__ __device__ constexpr int lin_stage_bytes(int bn) { return (kTileN + bn) * kKBlock; }
-__host__ __device__ constexpr int lin_stages(int bn) { return bn >= 256 ? 4 : bn >= 128 ? 6 : 8; }
+__host__ __device__ constexpr int lin_stages(int bn) { return bn >= 256 ? 4 : bn >= 128 ? 3 : bn >= 64 ? 4 : 5; }
 __host__ __device__ constexpr int lin_smem(int bn) { return lin_stages(bn) * lin_stage_bytes(bn) + 1024; }
 __host__ __device__ constexpr int lin_tmem(int bn) { return 2 * bn < 32 ? 32 : 2 * bn; }
 
@@ -41,7 +41,7 @@ __device__ __forceinline__ float scaled(uint32_t acc, float s, float v, float b)
 }
 
 template <int BN, int DT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, BN < 256 ? 2 : 1)
 int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap,
                    const LinearArgs a, int split) {
   constexpr int ST = lin_stages(BN), SB = lin_stage_bytes(BN);
@@ -52,7 +52,7 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
   __shared__ uint32_t tslot;
   const uint32_t ring = (smem_addr(dyn) + 1023) & ~1023u;
   const uint32_t full = smem_addr(bars), empty = full + 8 * ST, accf = empty + 8 * ST, acce = accf + 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     prefetch_map(&wmap);
     prefetch_map(&qmap);
@@ -80,7 +80,7 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
   const int kb1 = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / split);
   const int first = static_cast<int>(blockIdx.x) / split, step = static_cast<int>(gridDim.x) / split;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // Copies: a stage is refilled once the matrix instructions that read it
     // are done.
     int it = 0, sent = 0;
@@ -93,9 +93,12 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(full + 8 * st, SB);
-        tma_load(ring + st * SB, &wmap, kb * kKBlock, n0, full + 8 * st);
-        tma_load(ring + st * SB + kTileN * kKBlock, &qmap, kb * kKBlock, m0, full + 8 * st);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(full + 8 * st, SB);
+          tma_load(ring + st * SB, &wmap, kb * kKBlock, n0, full + 8 * st);
+          tma_load(ring + st * SB + kTileN * kKBlock, &qmap, kb * kKBlock, m0, full + 8 * st);
+        }
+        __syncwarp();
         sent = it + 1;
       }
     }
@@ -103,9 +106,10 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
     // block ends.
     if (!ok)
       for (int i = sent > ST ? sent - ST : 0; i < sent; ++i) mbar_wait(full + 8 * (i % ST), (i / ST) & 1);
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     // 32-bit sums of signed bytes, BN columns, 128 lanes.
     constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileN >> 4) << 24);
+    const uint64_t desc0 = smem_desc(ring, 16, 1024);
     int it = 0, n = 0;
     bool ok = true;
     for (int tile = first; ok && tile < a.tiles; tile += step, ++n) {
@@ -119,14 +123,18 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
           break;
         }
         tc_fence_after();
-        const uint64_t da = smem_desc(ring + st * SB, 16, 1024);
-        const uint64_t db = smem_desc(ring + st * SB + kTileN * kKBlock, 16, 1024);
+        if (elect_one()) {
+          const uint64_t da = desc0 + static_cast<uint64_t>(st * (SB >> 4));
+          const uint64_t db = da + (kTileN * kKBlock >> 4);
 #pragma unroll
-        for (int k = 0; k < kKBlock / 32; ++k)
-          mma_i8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, kb > kb0 || k > 0);
-        mma_commit(empty + 8 * st);
+          for (int k = 0; k < kKBlock / 32; ++k)
+            mma_i8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, kb > kb0 || k > 0);
+          mma_commit(empty + 8 * st);
+        }
+        __syncwarp();
       }
-      mma_commit(accf + 8 * buf);
+      if (elect_one()) mma_commit(accf + 8 * buf);
+      __syncwarp();
     }
   } else if (warp >= 2) {
     const int quad = warp & 3;  // the tensor-memory lanes that this warp may read
@@ -222,20 +230,37 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
   if (split > 1) {
     __syncwarp();
     cluster_sync();
-    if (warp >= 2) {
-      const int quad = warp & 3;
-      const int n0 = (first % a.ntiles) * kTileN, m0 = (first / a.ntiles) * BN;
-      const int ch = n0 + quad * 32 + lane;
-      const int cols = min(BN, a.M - m0);
-      const bool nok = ch < a.N;
-      const float vn = nok ? __ldg(a.v + ch) : 0.0f;
-      const float b = nok && a.bias != nullptr ? load1<DT>(a.bias + ch) : 0.0f;
-      const uint32_t at = ring + (quad * 32 + lane) * 4;
-      for (int c = rank; c < cols; c += split) {
-        uint32_t acc = 0;
-        for (int r = 0; r < split; ++r) acc += peer_ld(peer_addr(at + c * 512, r));
-        if (nok)
-          a.y[static_cast<int64_t>(m0 + c) * a.N + ch] = static_cast<uint16_t>(pack2<DT>(scaled(acc, sm[0][c], vn, b), 0.0f));
+    // Four channels a lane, a column a warp and step.
+    const int n0 = (first % a.ntiles) * kTileN, m0 = (first / a.ntiles) * BN;
+    const int cols = min(BN, a.M - m0), ch = n0 + 4 * lane;
+    if (ch < a.N) {
+      float vn[4], b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        vn[j] = ch + j < a.N ? __ldg(a.v + ch + j) : 0.0f;
+        b[j] = a.bias != nullptr && ch + j < a.N ? load1<DT>(a.bias + ch + j) : 0.0f;
+      }
+      for (int c = rank + split * warp; c < cols; c += split * (kThreads / 32)) {
+        uint4 p[8];
+        peer_ld_all(ring + c * 512 + lane * 16, split, p);
+        const float s = sm[0][c];
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t acc = 0;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) acc += word(p[r], j);
+          f[j] = scaled(acc, s, vn[j], b[j]);
+        }
+        uint16_t* y = a.y + static_cast<int64_t>(m0 + c) * a.N + ch;
+        const uint2 o = make_uint2(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]));
+        if (a.N % 4 == 0) {
+          st8(y, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (ch + j < a.N) y[j] = static_cast<uint16_t>((j < 2 ? o.x : o.y) >> (16 * (j & 1)));
+        }
       }
     }
     __syncwarp();
@@ -261,7 +286,7 @@ static cudaError_t launch_linear(const void* q, const void* w, LinearArgs a, int
   if (e != cudaSuccess) return e;
   a.ntiles = (a.N + kTileN - 1) / kTileN;
   a.tiles = a.ntiles * ((a.M + BN - 1) / BN);
-  const int grid = split > 1 ? a.tiles * split : std::min(a.tiles, device_info().sms);
+  const int grid = split > 1 ? a.tiles * split : std::min(a.tiles, device_info().sms * (BN < 256 ? 2 : 1));
   return launch_cluster(int8_linear_kernel<BN, DT>, dim3(grid), dim3(kThreads), lin_smem(BN), split, st, wmap, qmap, a,
                         split);
 }

@@ -1,52 +1,294 @@
 // Weight gradient from 8-bit checkpoints:
 //   dw[n, k] = sum_t dy[t, n] (q[t, k] s[t])
 // over the tokens t, with the codes and scales that the forward product read.
+//
+// The sum runs along the rows of both operands, so both enter the matrix
+// instruction with their k index (the token) outermost: dy as it lies, by TMA;
+// the codes after groups of four warps have turned a stage's 64 tokens x 128 channels
+// into 16-bit floats, each value q s rounded once (the codes times a scale of
+// their own token fit no exponent of the instruction).  The sum is fp32.
+//
+// A tile is 128 channels (tensor-memory lanes) by BN columns of dy.  For an
+// adapter's few columns the kernel reads the codes once at memory speed; for a
+// full weight it is bound by the matrix instructions.  Few tiles are split
+// along the tokens over a cluster, whose parts are added in order of rank
+// through distributed shared memory: the order is fixed by the sizes alone.
 #include "int8_common.cuh"
+#include "tc_device.cuh"
+
+#include <algorithm>
 
 namespace afb {
 
 struct WgradArgs {
-  const uint16_t* dy;  // [T, N]
-  const int8_t* q;     // [T, K]
-  const float* s;      // [T]
-  uint16_t* dw;        // [N, K]
+  const float* s;  // [T]
+  uint16_t* dw;    // [N, K]
   int T, N, K;
+  int ktiles;
 };
 
-// 64 x 64 outputs a block of 256 threads, 16 tokens a step, fp32.
+constexpr int kTok = 64;  // tokens of a stage
+constexpr int kCh = 128;  // channels of a tile
+
+// A stage: the converted operand, dy in chunks of 64 columns, the codes.
+__host__ __device__ constexpr int wg_chunks(int bn) { return bn < 64 ? 1 : bn / 64; }
+__host__ __device__ constexpr int wg_conv_bytes() { return kCh * kTok * 2; }
+__host__ __device__ constexpr int wg_stage_bytes(int bn) { return wg_conv_bytes() + wg_chunks(bn) * kTok * 128 + kTok * kCh; }
+__host__ __device__ constexpr int wg_stages(int bn) { return bn >= 128 ? 4 : 3; }
+// Groups of four warps that convert, one for each stage of the ring, and then
+// write the results.  Sixteen warps on one stage after another took 0.58 us a
+// stage, the latency of one pass from wait to arrival.  A group meets its stage
+// in every phase: a wait by parity may be one phase behind its barrier, not two.
+__host__ __device__ constexpr int wg_groups(int bn) { return wg_stages(bn); }
+__host__ __device__ constexpr int wg_threads(int bn) { return 64 + 128 * wg_groups(bn); }
+__host__ __device__ constexpr int wg_smem(int bn) { return wg_stages(bn) * wg_stage_bytes(bn) + 1024; }
+__host__ __device__ constexpr int wg_tmem(int bn) { return bn < 32 ? 32 : bn; }
+
+// Sixteen codes to two 16-byte pieces of the 16-bit type, times the scale.
 template <int DT>
-__global__ void __launch_bounds__(256) int8_wgrad_kernel(const WgradArgs a) {
-  __shared__ float dy[16][65], x[16][65];
+__device__ __forceinline__ void convert16(const uint4 q, float s, uint4& lo, uint4& hi) {
+  const f2_t s2 = splat2(s);
+  uint32_t o[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w = word(q, j) ^ 0x80808080u;  // code + 128 in each byte
+    // 2^23 + 128 + code, then minus 2^23 + 128
+    const f2_t a = f2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)),
+                      __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)));
+    const f2_t b = f2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)),
+                      __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)));
+    const f2_t base = splat2(8388736.0f);
+    o[2 * j] = pack2<DT>(mul2(sub2(a, base), s2));
+    o[2 * j + 1] = pack2<DT>(mul2(sub2(b, base), s2));
+  }
+  lo = make_uint4(o[0], o[1], o[2], o[3]);
+  hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+template <int BN, int DT>
+__global__ void __launch_bounds__(wg_threads(BN), BN <= 64 ? 2 : 1)
+int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
+                  const WgradArgs a, int split) {
+  constexpr int ST = wg_stages(BN), SB = wg_stage_bytes(BN), CH = wg_chunks(BN), G = wg_groups(BN);
+  constexpr int kGOff = wg_conv_bytes(), kQOff = kGOff + CH * kTok * 128;
+  extern __shared__ uint8_t dyn[];
+  __shared__ __align__(8) uint64_t bars[3 * ST + 1];
+  __shared__ uint32_t tslot;
+  const uint32_t ring = (smem_addr(dyn) + 1023) & ~1023u;
+  const uint32_t full = smem_addr(bars), conv = full + 8 * ST, empty = conv + 8 * ST, accf = empty + 8 * ST;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    prefetch_map(&qmap);
+    prefetch_map(&gmap);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(conv + 8 * i, 4);
+      mbar_init(empty + 8 * i, 1);
+    }
+    mbar_init(accf, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(smem_addr(&tslot), wg_tmem(BN));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tslot;
   pdl_wait();
   pdl_trigger();
-  const int n0 = blockIdx.y * 64, k0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int t0 = 0; t0 < a.T; t0 += 16) {
-    for (int i = threadIdx.x; i < 16 * 64; i += 256) {
-      const int t = t0 + i / 64, c = i % 64;
-      dy[i / 64][c] = t < a.T && n0 + c < a.N ? load1<DT>(a.dy + static_cast<int64_t>(t) * a.N + n0 + c) : 0.0f;
-      x[i / 64][c] = t < a.T && k0 + c < a.K
-                         ? static_cast<float>(a.q[static_cast<int64_t>(t) * a.K + k0 + c]) * __ldg(a.s + t) : 0.0f;
+
+  const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int tile = static_cast<int>(blockIdx.x) / split;
+  const int k0 = (tile % a.ktiles) * kCh, n0 = (tile / a.ktiles) * BN;
+  const int blocks = (a.T + kTok - 1) / kTok;
+  const int b0 = static_cast<int>(static_cast<int64_t>(blocks) * rank / split);
+  const int nb = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / split) - b0;
+
+  bool done = false;  // the accumulator holds this part's sum
+  if (warp == 0) {
+    int sent = 0;
+    bool ok = true;
+    for (int it = 0; it < nb; ++it) {
+      const int st = it % ST;
+      const uint32_t base = ring + st * SB;
+      if (it >= ST && !mbar_wait(empty + 8 * st, ((it / ST) - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      if (elect_one()) {
+        mbar_arrive_expect_tx(full + 8 * st, SB - wg_conv_bytes());
+        tma_load(base + kQOff, &qmap, k0, (b0 + it) * kTok, full + 8 * st);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          tma_load(base + kGOff + c * kTok * 128, &gmap, n0 + 64 * c, (b0 + it) * kTok, full + 8 * st);
+      }
+      __syncwarp();
+      sent = it + 1;
     }
-    __syncthreads();
+    if (!ok)  // copies still in flight land before the block ends
+      for (int i = sent > ST ? sent - ST : 0; i < sent; ++i) mbar_wait(full + 8 * (i % ST), (i / ST) & 1);
+  } else if (warp == 1) {
+    // fp32 sums; both operands 16-bit floats, outermost along k (bits 15, 16).
+    constexpr uint32_t type = DT == kBf16 ? 1u : 0u;
+    constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) |
+                               (uint32_t(BN >> 3) << 17) | (uint32_t(kCh >> 4) << 24);
+    const uint64_t desc0 = smem_desc(ring, kTok * 128, 1024);
+    for (int it = 0; it < nb; ++it) {
+      const int st = it % ST;
+      if (!mbar_wait(full + 8 * st, (it / ST) & 1) || !mbar_wait(conv + 8 * st, (it / ST) & 1)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t da = desc0 + static_cast<uint64_t>(st * (SB >> 4)), db = da + (kGOff >> 4);
 #pragma unroll
-    for (int t = 0; t < 16; ++t)
+        for (int k = 0; k < kTok / 16; ++k)  // 16 tokens: two groups of 8 rows of 128 bytes
+          mma_f16(tmem, da + k * (2048 >> 4), db + k * (2048 >> 4), idesc, it > 0 || k > 0);
+        mma_commit(empty + 8 * st);
+      }
+      __syncwarp();
+    }
+    if (elect_one()) mma_commit(accf);
+    __syncwarp();
+  } else if (warp >= 2) {
+    // A warp converts 16 tokens of a stage, four at a time: 8 lanes read a
+    // token's 128 codes.  Lane l keeps the scale of the warp's token l % 16, in
+    // this stage of the group or its next one (l / 16), and asks for the two
+    // after them when these begin, so that no stage waits for the load.
+    const int w = (warp - 2) & 3, part = lane & 7;
+    auto scale_at = [&](int it) {
+      const int at = it + (lane >> 4) * G;
+      const int t = (b0 + at) * kTok + ((lane >> 2) & 3) * 16 + w * 4 + (lane & 3);
+      return at < nb && t < a.T ? __ldg(a.s + t) : 0.0f;
+    };
+    const int g = (warp - 2) >> 2;
+    float now = 0.0f, next = scale_at(g);
+    int half = 0;
+    for (int it = g; it < nb; it += G, half ^= 16) {
+      const int st = it % ST;
+      const uint32_t base = ring + st * SB;
+      if (half == 0) {
+        now = next;
+        next = scale_at(it + 2 * G);
+      }
+      // full implies that the stage's last readers are done
+      if (!mbar_wait(full + 8 * st, (it / ST) & 1)) break;
+      uint4 code[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) code[i] = lds16a(base + kQOff + (i * 16 + w * 4 + (lane >> 3)) * kCh + part * 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(dy[t][ty + 16 * i], x[t][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+      for (int i = 0; i < 4; ++i) {
+        const int t = i * 16 + w * 4 + (lane >> 3);
+        const float sc = __shfl_sync(kFull, now, half + i * 4 + (lane >> 3));
+        uint4 lo, hi;
+        convert16<DT>(code[i], sc, lo, hi);
+        // chunk of 64 channels, row of the token, 16-byte pieces swizzled by the row
+        const uint32_t row = base + (part >> 2) * (kTok * 128) + t * 128;
+        const uint32_t p0 = ((2 * (part & 3)) ^ (t & 7)) * 16;
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + p0), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (p0 ^ 16)), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(conv + 8 * st);
+    }
+    done = mbar_wait(accf, 0);
+    tc_fence_after();
   }
+
+  const int quad = warp & 3, group = (warp - 2) >> 2;  // lanes, and every G-th block of columns
+  const int ch = k0 + quad * 32 + lane;
+  const int cols = min(BN, a.N - n0);
+  const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+  const uint32_t at = ring + (quad * 32 + lane) * 4;
+  if (warp >= 2 && done) {
+#pragma unroll 1
+    for (int c = 16 * group; c < cols; c += 16 * G) {
+      uint32_t v[16];
+      tmem_ld16(trow + c, v);
+      tmem_ld_wait();
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + ty + 16 * i, k = k0 + tx + 16 * j;
-      if (n < a.N && k < a.K)
-        a.dw[static_cast<int64_t>(n) * a.K + k] = static_cast<uint16_t>(pack2<DT>(acc[i][j], 0.0f));
+      for (int i = 0; i < 16; ++i) {
+        if (nb == 0) v[i] = 0;
+        if (split > 1) {
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (c + i) * 512), "r"(v[i]) : "memory");
+        } else if (ch < a.K && c + i < cols) {
+          a.dw[static_cast<int64_t>(n0 + c + i) * a.K + ch] = static_cast<uint16_t>(pack2<DT>(__uint_as_float(v[i]), 0.0f));
+        }
+      }
     }
+  }
+  if (split > 1) {
+    __syncwarp();
+    cluster_sync();
+    // Four channels a lane, a column a warp and step.
+    if (warp >= 2 && k0 + 4 * lane < a.K) {
+      for (int c = rank + split * (warp - 2); c < cols; c += split * 4 * G) {
+        uint4 p[8];
+        peer_ld_all(ring + c * 512 + lane * 16, split, p);
+        float f[4] = {};
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[j] += __uint_as_float(word(p[r], j));
+        st8(a.dw + static_cast<int64_t>(n0 + c) * a.K + k0 + 4 * lane, make_uint2(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3])));
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_free(tmem, wg_tmem(BN));
+  }
 }
+
+template <int BN, int DT>
+static cudaError_t launch_wgrad(const void* dy, const void* q, WgradArgs a, int split, cudaStream_t st) {
+  CUtensorMap qmap, gmap;
+  cudaError_t e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, q, a.K, a.T, a.K, kCh, kTok);
+  if (e == cudaSuccess)
+    e = make_map(&gmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B, dy, a.N, a.T,
+                 static_cast<uint64_t>(a.N) * 2, 64, kTok);
+  if (e == cudaSuccess) e = ensure_smem(int8_wgrad_kernel<BN, DT>, wg_smem(BN));
+  if (e != cudaSuccess) return e;
+  a.ktiles = (a.K + kCh - 1) / kCh;
+  const int tiles = a.ktiles * ((a.N + BN - 1) / BN);
+  return launch_cluster(int8_wgrad_kernel<BN, DT>, dim3(tiles * split), dim3(wg_threads(BN)), wg_smem(BN), split, st, qmap,
+                        gmap, a, split);
+}
+
+// Columns of a tile and parts along the tokens: the narrowest tile that holds
+// all columns, up to 128, or 256 where that still gives every multiprocessor a
+// tile; what is left idle goes to parts of at least two stages.
+static void wgrad_shape(int T, int N, int K, int sms, int* bn, int* split) {
+  const int64_t kt = (K + kCh - 1) / kCh;
+  auto tiles = [&](int b) { return kt * ((N + b - 1) / b); };
+  int b = 16;
+  while (b < 256 && b < N && (b < 128 || tiles(2 * b) >= sms)) b *= 2;
+  const int blocks = (T + kTok - 1) / kTok;
+  int s = 1;
+  while (s < 8 && b < 256 && tiles(b) * s * 2 <= sms && blocks / (2 * s) >= 2) s *= 2;
+  *bn = b;
+  *split = s;
+}
+
+template <int DT>
+static cudaError_t wgrad(const void* dy, const void* q, const WgradArgs& a, cudaStream_t st) {
+  const DeviceInfo& d = device_info();
+  if (d.error != cudaSuccess) return d.error;
+  int bn, split;
+  wgrad_shape(a.T, a.N, a.K, d.sms, &bn, &split);
+  switch (bn) {
+    case 16: return launch_wgrad<16, DT>(dy, q, a, split, st);
+    case 32: return launch_wgrad<32, DT>(dy, q, a, split, st);
+    case 64: return launch_wgrad<64, DT>(dy, q, a, split, st);
+    case 128: return launch_wgrad<128, DT>(dy, q, a, split, st);
+    default: return launch_wgrad<256, DT>(dy, q, a, split, st);
+  }
+}
+
+cudaError_t read_status_int8_wgrad(int* status, bool clear) { return tu_status(status, clear); }
 
 }  // namespace afb
 
@@ -61,10 +303,13 @@ extern "C" int afb_int8_wgrad(const void* dy, const void* q, const void* s, void
       !check_dtype(dtype) || !check_ptrs({dw}, {"dw"}))
     return g.fail();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (rows != 0 && (!check_ptrs({dy, q}, {"dy", "q"}) || !check_ptr4(s, "s"))) return g.fail();
-  WgradArgs a{static_cast<const uint16_t*>(dy), static_cast<const int8_t*>(q), static_cast<const float*>(s),
-              static_cast<uint16_t*>(dw), static_cast<int>(rows), static_cast<int>(N), static_cast<int>(K)};
-  const dim3 grid(static_cast<unsigned>((K + 63) / 64), static_cast<unsigned>((N + 63) / 64));
-  return g.done(dtype == kBf16 ? launch_pdl(int8_wgrad_kernel<kBf16>, grid, dim3(256), 0, st, a)
-                               : launch_pdl(int8_wgrad_kernel<kFp16>, grid, dim3(256), 0, st, a));
+  if (rows == 0) return g.done(cudaMemsetAsync(dw, 0, static_cast<size_t>(N) * K * 2, st));
+  if (!check_ptrs({dy, q}, {"dy", "q"}) || !check_ptr4(s, "s")) return g.fail();
+  WgradArgs a{};
+  a.s = static_cast<const float*>(s);
+  a.dw = static_cast<uint16_t*>(dw);
+  a.T = static_cast<int>(rows);
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  return g.done(dtype == kBf16 ? wgrad<kBf16>(dy, q, a, st) : wgrad<kFp16>(dy, q, a, st));
 }

@@ -33,6 +33,17 @@ inline cudaError_t make_map(CUtensorMap* map, CUtensorMapDataType type, CUtensor
 }
 
 // -------------------------------------------------------------- device side --
+// The warp's index, the same register in all its lanes for the compiler too.
+__device__ __forceinline__ int warp_index() { return __shfl_sync(kFull, static_cast<int>(threadIdx.x >> 5), 0); }
+// True in one lane of a converged warp.  Copies and matrix instructions take
+// their operands from uniform registers: issued under this predicate by a warp
+// whose lanes all run the loop, a stage's four instructions take about half
+// the time of the same loop run by lane 0 alone.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }
@@ -131,10 +142,16 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ uint32_t peer_ld(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
+__device__ __forceinline__ uint4 peer_ld16(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
+  return r;
+}
+// The 16 bytes at `addr` of every CTA of a cluster of up to 8; zero above it.
+// All are asked for before the first is used.
+__device__ __forceinline__ void peer_ld_all(uint32_t addr, int split, uint4 (&p)[8]) {
+#pragma unroll
+  for (int r = 0; r < 8; ++r) p[r] = r < split ? peer_ld16(peer_addr(addr, r)) : make_uint4(0, 0, 0, 0);
 }
 
 // Launch with a cluster of `cluster` CTAs along x.
