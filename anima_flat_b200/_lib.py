@@ -50,6 +50,7 @@ SIGNATURES: dict[str, tuple] = {
     "afb_gelu_int8_bwd": (_P, _P, _P, _P, _I, _I, c_int, _P),
     "afb_int8_restore": (_P, _P, _P, _I, _I, c_int, _P),
     "afb_int8_linear": (_P, _P, _P, _P, _P, _P, _I, _I, _I, c_int, _P),
+    "afb_int8_linear_x": (_P, _P, _P, _P, _P, _P, _I, _I, _I, c_int, _P, ctypes.c_size_t, _P),
     "afb_int8_wgrad": (_P, _P, _P, _P, _I, _I, _I, c_int, _P),
     "afb_sandwich_norm": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F, c_int, _P),
     "afb_sandwich_norm_int8": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F, c_int, _P),

@@ -105,6 +105,11 @@ inline bool check(bool ok, const std::string& msg) {
   if (!ok) set_error(msg);
   return ok;
 }
+// The same for messages that are plain text: no string is made unless it fails.
+inline bool check(bool ok, const char* msg) {
+  if (!ok) set_error(msg);
+  return ok;
+}
 
 // Row-kernel shape check: batch >= 0, seq >= 1, dim a multiple of 8 up to
 // kMaxRowDim.
@@ -122,8 +127,8 @@ inline bool check_ptrs(std::initializer_list<const void*> ps, std::initializer_l
   auto n = names.begin();
   for (const void* p : ps) {
     const char* nm = (n != names.end()) ? *n++ : "pointer";
-    if (!check(p != nullptr, std::string(nm) + " is null")) return false;
-    if (!check(aligned(p, 16), std::string(nm) + " is not 16-byte aligned")) return false;
+    if (p == nullptr) return check(false, std::string(nm) + " is null");
+    if (!aligned(p, 16)) return check(false, std::string(nm) + " is not 16-byte aligned");
   }
   return true;
 }

@@ -119,6 +119,10 @@ __device__ __forceinline__ f2_t code_pair(uint32_t w, int j) {
                 : f2(static_cast<float>(static_cast<int8_t>(v >> 16)), static_cast<float>(v >> 24));
 }
 
+// Codes and scales of x, or of x * cols where cols is not null (int8_quant.cu).
+cudaError_t quantize_rows(const void* x, const void* cols, int8_t* q, float* s, int64_t rows, int64_t K, int dtype,
+                          cudaStream_t st);
+
 inline bool check_dtype(int dtype) { return check(dtype == kBf16 || dtype == kFp16, "dtype must be 0 (bf16) or 1 (fp16)"); }
 
 }  // namespace afb

@@ -20,7 +20,7 @@ namespace afb {
 
 struct LinearArgs {
   const float* s;        // [M]
-  const float* v;        // [N]
+  const float* v;        // [N] or null (1)
   const uint16_t* bias;  // [N] or null
   uint16_t* y;           // [M, N]
   int M, N, K;
@@ -36,6 +36,7 @@ __host__ __device__ constexpr int lin_stages(int bn) { return bn >= 256 ? 4 : bn
 __host__ __device__ constexpr int lin_smem(int bn) { return lin_stages(bn) * lin_stage_bytes(bn) + 1024; }
 __host__ __device__ constexpr int lin_tmem(int bn) { return 2 * bn < 32 ? 32 : 2 * bn; }
 
+__device__ __forceinline__ float scale_of(const LinearArgs& a, int n) { return a.v != nullptr ? __ldg(a.v + n) : 1.0f; }
 __device__ __forceinline__ float scaled(uint32_t acc, float s, float v, float b) {
   return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(acc)), s), v), b);
 }
@@ -147,7 +148,7 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
       const int n0 = (tile % a.ntiles) * kTileN, m0 = (tile / a.ntiles) * BN;
       const int ch = n0 + quad * 32 + lane;
       const bool nok = ch < a.N;
-      const float vn = nok ? __ldg(a.v + ch) : 0.0f;
+      const float vn = nok ? scale_of(a, ch) : 0.0f;
       const float b = nok && a.bias != nullptr ? load1<DT>(a.bias + ch) : 0.0f;
       for (int i = et; i < BN; i += 128) sm[buf][i] = m0 + i < a.M ? __ldg(a.s + m0 + i) : 0.0f;
       named_bar_sync(1, 128);
@@ -237,7 +238,7 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
       float vn[4], b[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        vn[j] = ch + j < a.N ? __ldg(a.v + ch + j) : 0.0f;
+        vn[j] = ch + j < a.N ? scale_of(a, ch + j) : 0.0f;
         b[j] = a.bias != nullptr && ch + j < a.N ? load1<DT>(a.bias + ch + j) : 0.0f;
       }
       for (int c = rank + split * warp; c < cols; c += split * (kThreads / 32)) {
@@ -327,18 +328,20 @@ cudaError_t read_status_int8_linear(int* status, bool clear) { return tu_status(
 
 using namespace afb;
 
-extern "C" int afb_int8_linear(const void* q, const void* s, const void* w, const void* v, const void* bias, void* y,
-                               int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
-  ApiGuard g("afb_int8_linear");
-  if (!check(M >= 0 && M <= (1 << 30), "M must be in [0, 2^30]") || !check(N >= 1 && N <= (1 << 30), "N must be in [1, 2^30]") ||
-      !check(K >= 16 && K % 16 == 0 && K <= 131072, "K must be a multiple of 16 in [16, 131072], got " + std::to_string(K)) ||
-      !check_dtype(dtype))
-    return g.fail();
-  if (M == 0) return 0;
-  if (!check_ptrs({q, w}, {"q", "w"}) || !check_ptr4(s, "s") || !check_ptr4(v, "v") ||
-      !check(y != nullptr && aligned(y, 16), "y is null or not 16-byte aligned") ||
-      !check(aligned(bias, 2), "bias is not 2-byte aligned"))
-    return g.fail();
+static bool check_linear(const void* w, const void* v, const void* bias, void* y, int64_t M, int64_t N, int64_t K,
+                         int64_t most_k, int dtype) {
+  return check(M >= 0 && M <= (1 << 30), "M must be in [0, 2^30]") &&
+         check(N >= 1 && N <= (1 << 30), "N must be in [1, 2^30]") &&
+         check(((M + 15) / 16) * ((N + kTileN - 1) / kTileN) <= (1 << 27), "M * N is too large") &&
+         check(K >= 16 && K % 16 == 0 && K <= most_k,
+               "K must be a multiple of 16 in [16, " + std::to_string(most_k) + "], got " + std::to_string(K)) &&
+         check_dtype(dtype) &&
+         (M == 0 || (check_ptrs({w, y}, {"w", "y"}) && check(aligned(v, 4), "v is not 4-byte aligned") &&
+                     check(aligned(bias, 2), "bias is not 2-byte aligned")));
+}
+
+static cudaError_t run_linear(const void* q, const void* s, const void* w, const void* v, const void* bias, void* y,
+                              int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
   LinearArgs a{};
   a.s = static_cast<const float*>(s);
   a.v = static_cast<const float*>(v);
@@ -347,7 +350,31 @@ extern "C" int afb_int8_linear(const void* q, const void* s, const void* w, cons
   a.M = static_cast<int>(M);
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
-  if (!check(((M + 15) / 16) * ((N + kTileN - 1) / kTileN) <= (1 << 27), "M * N is too large")) return g.fail();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return g.done(dtype == kBf16 ? linear<kBf16>(q, w, a, st) : linear<kFp16>(q, w, a, st));
+  return dtype == kBf16 ? linear<kBf16>(q, w, a, st) : linear<kFp16>(q, w, a, st);
+}
+
+extern "C" int afb_int8_linear(const void* q, const void* s, const void* w, const void* v, const void* bias, void* y,
+                               int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
+  ApiGuard g("afb_int8_linear");
+  if (!check_linear(w, v, bias, y, M, N, K, 131072, dtype)) return g.fail();
+  if (M == 0) return 0;
+  if (!check_ptrs({q}, {"q"}) || !check_ptr4(s, "s") || !check_ptr4(v, "v")) return g.fail();
+  return g.done(run_linear(q, s, w, v, bias, y, M, N, K, dtype, stream));
+}
+
+extern "C" int afb_int8_linear_x(const void* x, const void* cols, const void* w, const void* v, const void* bias,
+                                 void* y, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  ApiGuard g("afb_int8_linear_x");
+  if (!check_linear(w, v, bias, y, M, N, K, 16384, dtype)) return g.fail();
+  if (M == 0) return 0;
+  if (!check_ptrs({x, workspace}, {"x", "workspace"}) || !check(aligned(cols, 16), "cols is not 16-byte aligned") ||
+      !check(workspace_bytes >= static_cast<size_t>(M) * (K + 4), "workspace too small"))
+    return g.fail();
+  int8_t* q = static_cast<int8_t*>(workspace);
+  float* s = reinterpret_cast<float*>(q + M * K);
+  const cudaError_t e = quantize_rows(x, cols, q, s, M, K, dtype, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return g.done(e);
+  return g.done(run_linear(q, s, w, v, bias, y, M, N, K, dtype, stream));
 }

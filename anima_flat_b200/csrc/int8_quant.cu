@@ -153,6 +153,19 @@ static cudaError_t launch_quant(const QuantArgs& a, cudaStream_t st) {
   }
 }
 
+cudaError_t quantize_rows(const void* x, const void* cols, int8_t* q, float* s, int64_t rows, int64_t K, int dtype,
+                          cudaStream_t st) {
+  QuantArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.cols = static_cast<const float*>(cols);
+  a.q = q;
+  a.s = s;
+  a.rows = rows;
+  a.K = static_cast<int>(K);
+  if (cols != nullptr) return dtype == kBf16 ? launch_quant<kBf16, kCols>(a, st) : launch_quant<kFp16, kCols>(a, st);
+  return dtype == kBf16 ? launch_quant<kBf16, kPlain>(a, st) : launch_quant<kFp16, kPlain>(a, st);
+}
+
 // ------------------------------------------------------------ restore, GELU' --
 struct RestoreArgs {
   const int8_t* q;     // [rows, K]
@@ -237,17 +250,8 @@ extern "C" int afb_rowquant_int8(const void* x, const void* cols, void* q, void*
   if (!check_ptrs({x, q}, {"x", "q"}) || !check_ptr4(s, "s") ||
       !check(cols == nullptr || aligned(cols, 16), "cols is not 16-byte aligned"))
     return g.fail();
-  QuantArgs a{};
-  a.x = static_cast<const uint16_t*>(x);
-  a.cols = static_cast<const float*>(cols);
-  a.q = static_cast<int8_t*>(q);
-  a.s = static_cast<float*>(s);
-  a.rows = rows;
-  a.K = static_cast<int>(K);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cols != nullptr)
-    return g.done(dtype == kBf16 ? launch_quant<kBf16, kCols>(a, st) : launch_quant<kFp16, kCols>(a, st));
-  return g.done(dtype == kBf16 ? launch_quant<kBf16, kPlain>(a, st) : launch_quant<kFp16, kPlain>(a, st));
+  return g.done(quantize_rows(x, cols, static_cast<int8_t*>(q), static_cast<float*>(s), rows, K, dtype,
+                              static_cast<cudaStream_t>(stream)));
 }
 
 extern "C" int afb_gelu_int8(const void* x, void* q, void* s, void* c, void* cs, int64_t rows, int64_t K,

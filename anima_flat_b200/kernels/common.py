@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import torch
 
+from .._lib import call
+
 BF16 = torch.bfloat16
 
 
@@ -51,14 +53,51 @@ def _check_same_device(*ts: torch.Tensor | None) -> None:
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError("CUDA tensors required")
-        if device is not None and t.device != device:
-            raise ValueError(f"tensors are on {device} and {t.device}")
-        device = t.device
+        d = t.get_device()
+        if d != device:
+            if d < 0 or not t.is_cuda:
+                raise ValueError("CUDA tensors required")
+            if device is not None:
+                raise ValueError(f"tensors are on devices {device} and {d}")
+            device = d
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned: a copy only where `t` is neither."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    """Contiguous and 16-byte aligned: a copy only where `t` is not."""
+    if t.is_contiguous():
+        return t if not t.data_ptr() & 15 else t.clone()
+    return t.contiguous()
+
+
+_Tensor, _Parameter = torch.Tensor, torch.nn.Parameter
+
+
+def _plain(*ts: torch.Tensor | None) -> bool:
+    """True where the launches may be called directly, without torch's dispatcher.
+
+    That is: ordinary tensors, outside compilation, dispatch modes (fake tensors,
+    tracing), function transforms and forward-mode differentiation, all of which
+    need the registered op.  A Python custom op costs about 40 us a call, several
+    times a small launch; the direct call about 6.
+    """
+    if (
+        torch.compiler.is_compiling()
+        or torch._C._len_torch_dispatch_stack()
+        or torch._C._functorch.peek_interpreter_stack() is not None
+        or torch.autograd.forward_ad._current_level >= 0
+    ):
+        return False
+    for t in ts:
+        if t is not None and type(t) is not _Tensor and type(t) is not _Parameter:
+            return False
+    return True
+
+
+def _launch(name: str, t: torch.Tensor, *args) -> None:
+    """Call entry point `name` on the current stream of the device of `t`."""
+    device = t.get_device()
+    if device == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(device))

@@ -28,8 +28,7 @@ from typing import NamedTuple
 
 import torch
 
-from .._lib import call
-from .common import HALF_TYPES, _check_half, _check_same_device, _dense, _stream
+from .common import HALF_TYPES, _check_half, _check_same_device, _dense, _launch, _plain
 
 __all__ = [
     "Int8Weight",
@@ -59,23 +58,88 @@ class Int8Weight(NamedTuple):
 
 
 # ------------------------------------------------------------------ launches --
-def _quant(x: torch.Tensor, cols: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+def _quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     K = x.shape[-1]
     rows = x.numel() // K
-    q = torch.empty(x.shape, dtype=I8, device=x.device)
-    s = torch.empty((rows, 1), dtype=F32, device=x.device)
-    call("afb_rowquant_int8", x.data_ptr(), None if cols is None else cols.data_ptr(), q.data_ptr(),
-         s.data_ptr(), rows, K, HALF_TYPES[x.dtype], _stream(x))
+    q, s = torch.empty_like(x, dtype=I8), x.new_empty((rows, 1), dtype=F32)
+    _launch("afb_rowquant_int8", x, x.data_ptr(), None, q.data_ptr(), s.data_ptr(), rows, K, HALF_TYPES[x.dtype])
     return q, s
 
 
 def _product(q, s, wq, ws, bias, dtype):
     K, N = q.shape[-1], wq.shape[0]
-    y = torch.empty((*q.shape[:-1], N), dtype=dtype, device=q.device)
-    call("afb_int8_linear", q.data_ptr(), s.data_ptr(), wq.data_ptr(), ws.data_ptr(),
-         None if bias is None else bias.data_ptr(), y.data_ptr(), q.numel() // K, N, K,
-         HALF_TYPES[dtype], _stream(q))
+    y = q.new_empty((*q.shape[:-1], N), dtype=dtype)
+    _launch("afb_int8_linear", q, q.data_ptr(), s.data_ptr(), wq.data_ptr(), ws.data_ptr(),
+            None if bias is None else bias.data_ptr(), y.data_ptr(), q.numel() // K, N, K, HALF_TYPES[dtype])
     return y
+
+
+def _quant_product(x, cols, wq, ws, bias):
+    """Quantize x, or x * cols, and multiply: one call, its codes in a workspace."""
+    K, N = x.shape[-1], wq.shape[0]
+    rows = x.numel() // K
+    y = x.new_empty((*x.shape[:-1], N))
+    nbytes = rows * (K + 4)
+    work = x.new_empty(nbytes, dtype=I8)
+    _launch("afb_int8_linear_x", x, x.data_ptr(), None if cols is None else cols.data_ptr(), wq.data_ptr(),
+            None if ws is None else ws.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), rows, N, K,
+            HALF_TYPES[x.dtype], work.data_ptr(), nbytes)
+    return y
+
+
+def _linear(x, wq, ws, wqt, bias):
+    return _quant_product(x, None, wq, ws, bias)
+
+
+def _linear_bwd(dy, ws, wqt):
+    return _quant_product(_dense(dy), ws, wqt, None, None)
+
+
+def _gelu(x):
+    K = x.shape[-1]
+    rows = x.numel() // K
+    q, c = torch.empty_like(x, dtype=I8), torch.empty_like(x, dtype=I8)
+    s, cs = x.new_empty((rows, 1), dtype=F32), x.new_empty((rows, 1), dtype=F32)
+    _launch("afb_gelu_int8", x, x.data_ptr(), q.data_ptr(), s.data_ptr(), c.data_ptr(), cs.data_ptr(), rows, K,
+            HALF_TYPES[x.dtype])
+    return q, s, c, cs
+
+
+def _gelu_bwd(dy, c, cs):
+    dx = torch.empty_like(dy)
+    K = dy.shape[-1]
+    _launch("afb_gelu_int8_bwd", dy, dy.data_ptr(), c.data_ptr(), cs.data_ptr(), dx.data_ptr(), dy.numel() // K, K,
+            HALF_TYPES[dy.dtype])
+    return dx
+
+
+def _restore(q, s, dtype):
+    y = torch.empty_like(q, dtype=dtype)
+    K = q.shape[-1]
+    _launch("afb_int8_restore", q, q.data_ptr(), s.data_ptr(), y.data_ptr(), q.numel() // K, K, HALF_TYPES[dtype])
+    return y
+
+
+def _wgrad(dy, q, s):
+    N, K = dy.shape[-1], q.shape[-1]
+    dw = dy.new_empty((N, K))
+    _launch("afb_int8_wgrad", dy, dy.data_ptr(), q.data_ptr(), s.data_ptr(), dw.data_ptr(), q.numel() // K, N, K,
+            HALF_TYPES[dy.dtype])
+    return dw
+
+
+class _LinearFn(torch.autograd.Function):
+    """int8_linear's gradient where the launches are called directly."""
+
+    @staticmethod
+    def forward(ctx, x, wq, ws, wqt, bias):
+        ctx.save_for_backward(ws, wqt)
+        return _linear(x, wq, ws, wqt, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return _linear_bwd(dy, *ctx.saved_tensors), None, None, None, None
 
 
 # ----------------------------------------------------------------- custom ops --
@@ -107,8 +171,7 @@ def _int8_linear(
     x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, wqt: torch.Tensor | None,
     bias: torch.Tensor | None,
 ) -> torch.Tensor:
-    q, s = _quant(x)
-    return _product(q, s, wq, ws, bias, x.dtype)
+    return _linear(x, wq, ws, wqt, bias)
 
 
 @_int8_linear.register_fake
@@ -118,10 +181,7 @@ def _(x, wq, ws, wqt, bias):
 
 @torch.library.custom_op("anima_flat_b200::int8_linear_bwd", mutates_args=())
 def _int8_linear_bwd(dy: torch.Tensor, ws: torch.Tensor, wqt: torch.Tensor) -> torch.Tensor:
-    dy = _dense(dy)
-    q, s = _quant(dy, ws)
-    one = torch.ones(wqt.shape[0], dtype=F32, device=dy.device)
-    return _product(q, s, wqt, one, None, dy.dtype)
+    return _linear_bwd(dy, ws, wqt)
 
 
 @_int8_linear_bwd.register_fake
@@ -146,13 +206,7 @@ torch.library.register_autograd(
 
 @torch.library.custom_op("anima_flat_b200::gelu_int8", mutates_args=())
 def _gelu_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    K = x.shape[-1]
-    rows = x.numel() // K
-    q, c = torch.empty(x.shape, dtype=I8, device=x.device), torch.empty(x.shape, dtype=I8, device=x.device)
-    s, cs = (torch.empty((rows, 1), dtype=F32, device=x.device) for _ in range(2))
-    call("afb_gelu_int8", x.data_ptr(), q.data_ptr(), s.data_ptr(), c.data_ptr(), cs.data_ptr(), rows, K,
-         HALF_TYPES[x.dtype], _stream(x))
-    return q, s, c, cs
+    return _gelu(x)
 
 
 @_gelu_int8.register_fake
@@ -164,11 +218,7 @@ def _(x):
 
 @torch.library.custom_op("anima_flat_b200::gelu_int8_bwd", mutates_args=())
 def _gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.Tensor:
-    dx = torch.empty_like(dy)
-    K = dy.shape[-1]
-    call("afb_gelu_int8_bwd", dy.data_ptr(), c.data_ptr(), cs.data_ptr(), dx.data_ptr(), dy.numel() // K, K,
-         HALF_TYPES[dy.dtype], _stream(dy))
-    return dx
+    return _gelu_bwd(dy, c, cs)
 
 
 @_gelu_int8_bwd.register_fake
@@ -178,11 +228,7 @@ def _(dy, c, cs):
 
 @torch.library.custom_op("anima_flat_b200::int8_restore", mutates_args=())
 def _int8_restore(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    y = torch.empty(q.shape, dtype=dtype, device=q.device)
-    K = q.shape[-1]
-    call("afb_int8_restore", q.data_ptr(), s.data_ptr(), y.data_ptr(), q.numel() // K, K, HALF_TYPES[dtype],
-         _stream(q))
-    return y
+    return _restore(q, s, dtype)
 
 
 @_int8_restore.register_fake
@@ -192,11 +238,7 @@ def _(q, s, dtype):
 
 @torch.library.custom_op("anima_flat_b200::int8_wgrad", mutates_args=())
 def _int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
-    N, K = dy.shape[-1], q.shape[-1]
-    dw = torch.empty((N, K), dtype=dy.dtype, device=dy.device)
-    call("afb_int8_wgrad", dy.data_ptr(), q.data_ptr(), s.data_ptr(), dw.data_ptr(), q.numel() // K, N, K,
-         HALF_TYPES[dy.dtype], _stream(dy))
-    return dw
+    return _wgrad(dy, q, s)
 
 
 @_int8_wgrad.register_fake
@@ -219,14 +261,19 @@ def _check_codes(q: torch.Tensor, s: torch.Tensor) -> None:
         raise ValueError(f"one scale per row of the codes is needed: {list(q.shape)} and {list(s.shape)}")
 
 
-def _check_weight(weight: Int8Weight, K: int) -> None:
-    q, s, qt = weight
-    if q.dtype != I8 or q.ndim != 2 or q.shape[1] != K or not q.shape[0]:
-        raise ValueError(f"the weight's codes must be torch.int8 [N, {K}], got {q.dtype} {list(q.shape)}")
-    if s.dtype != F32 or s.numel() != q.shape[0]:
-        raise ValueError(f"the weight's scales must be torch.float32 [{q.shape[0]}], got {s.dtype} {list(s.shape)}")
-    if qt is not None and (qt.dtype != I8 or qt.shape != (K, q.shape[0])):
-        raise ValueError(f"the transposed codes must be torch.int8 [{K}, {q.shape[0]}]")
+def _check_weight(wq, ws, bias, K: int, dtype: torch.dtype) -> torch.Tensor | None:
+    if wq.dtype != I8 or wq.ndim != 2 or wq.shape[1] != K or not wq.shape[0]:
+        raise ValueError(f"the weight's codes must be torch.int8 [N, {K}], got {wq.dtype} {list(wq.shape)}")
+    N = wq.shape[0]
+    if ws.dtype != F32 or ws.numel() != N:
+        raise ValueError(f"the weight's scales must be torch.float32 [{N}], got {ws.dtype} {list(ws.shape)}")
+    if bias is None:
+        return None
+    if bias.dtype != dtype or bias.numel() != N:
+        raise ValueError(f"bias must be {dtype} [{N}], got {bias.dtype} {list(bias.shape)}")
+    if bias.requires_grad and torch.is_grad_enabled():
+        raise ValueError("bias is a constant here: it must not require a gradient")
+    return bias.contiguous()
 
 
 # --------------------------------------------------------------------- public --
@@ -245,7 +292,8 @@ def rowquant_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     _check_same_device(x)
     _check_half("x", x)
     _check_cols("x", x)
-    return _rowquant_int8(_dense(x))
+    x = _dense(x)
+    return _quant(x) if _plain(x) else _rowquant_int8(x)
 
 
 def quantize_weight_int8(w: torch.Tensor, backward: bool = False) -> Int8Weight:
@@ -291,34 +339,33 @@ def int8_linear(
         ValueError: On tensors off CUDA, unsupported dtypes or shapes, a bias that
             requires a gradient, or an ``x`` that does without transposed codes.
     """
-    codes = not isinstance(x, torch.Tensor)
-    first = x[0] if codes else x
-    _check_same_device(first, *weight, bias)
-    if codes:
-        _check_codes(*x)
+    wq, ws, wqt = weight
+    if not isinstance(x, torch.Tensor):
+        q, s = x
+        _check_same_device(q, s, wq, ws, bias)
+        _check_codes(q, s)
         if dtype not in HALF_TYPES:
             raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
-        _check_same_device(first, x[1])
-    else:
-        _check_half("x", x)
-        _check_cols("x", x)
-        dtype = x.dtype
-    _check_weight(weight, first.shape[-1])
-    wq, ws, wqt = _dense(weight.q), weight.s.contiguous(), weight.qt
-    if bias is not None:
-        if bias.dtype != dtype or bias.numel() != wq.shape[0]:
-            raise ValueError(f"bias must be {dtype} [{wq.shape[0]}], got {bias.dtype} {list(bias.shape)}")
-        if bias.requires_grad and torch.is_grad_enabled():
-            raise ValueError("bias is a constant here: it must not require a gradient")
-        bias = bias.contiguous()
-    if codes:
-        return _int8_linear_codes(_dense(x[0]), x[1].contiguous(), wq, ws, bias, dtype)
-    if torch.is_grad_enabled() and x.requires_grad:
+        bias = _check_weight(wq, ws, bias, q.shape[-1], dtype)
+        q, s, wq, ws = _dense(q), s.contiguous(), _dense(wq), ws.contiguous()
+        product = _product if _plain(q, s, wq, ws, bias) else _int8_linear_codes
+        return product(q, s, wq, ws, bias, dtype)
+    _check_same_device(x, wq, ws, wqt, bias)
+    _check_half("x", x)
+    _check_cols("x", x)
+    bias = _check_weight(wq, ws, bias, x.shape[-1], x.dtype)
+    x, wq, ws = _dense(x), _dense(wq), _dense(ws)
+    grad = x.requires_grad and torch.is_grad_enabled()
+    if grad:
         if wqt is None:
             raise ValueError("the input gradient needs quantize_weight_int8(w, backward=True)")
+        if wqt.dtype != I8 or wqt.shape != (x.shape[-1], wq.shape[0]):
+            raise ValueError(f"the transposed codes must be torch.int8 [{x.shape[-1]}, {wq.shape[0]}]")
         _check_cols("the transposed weight", wqt)
-        wqt, ws = _dense(wqt), _dense(ws)
-    return _int8_linear(_dense(x), wq, ws, wqt, bias)
+        wqt = _dense(wqt)
+    if not _plain(x, wq, ws, wqt, bias):
+        return _int8_linear(x, wq, ws, wqt, bias)
+    return _LinearFn.apply(x, wq, ws, wqt, bias) if grad else _linear(x, wq, ws, wqt, bias)
 
 
 def gelu_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -337,7 +384,8 @@ def gelu_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor
     _check_same_device(x)
     _check_half("x", x)
     _check_cols("x", x)
-    return _gelu_int8(_dense(x))
+    x = _dense(x)
+    return _gelu(x) if _plain(x) else _gelu_int8(x)
 
 
 def gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.Tensor:
@@ -356,7 +404,8 @@ def gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.
     _check_codes(c, cs)
     if dy.shape != c.shape:
         raise ValueError(f"dy and the codes must match, got {list(dy.shape)} and {list(c.shape)}")
-    return _gelu_int8_bwd(_dense(dy), _dense(c), cs.contiguous())
+    dy, c, cs = _dense(dy), _dense(c), cs.contiguous()
+    return _gelu_bwd(dy, c, cs) if _plain(dy, c, cs) else _gelu_int8_bwd(dy, c, cs)
 
 
 def int8_restore(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -369,7 +418,8 @@ def int8_restore(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bf
     _check_codes(q, s)
     if dtype not in HALF_TYPES:
         raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
-    return _int8_restore(_dense(q), s.contiguous(), dtype)
+    q, s = _dense(q), s.contiguous()
+    return _restore(q, s, dtype) if _plain(q, s) else _int8_restore(q, s, dtype)
 
 
 def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
@@ -395,4 +445,6 @@ def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tens
     N = dy.shape[-1]
     if N % 8:  # the kernel's copies of dy need rows of a multiple of 16 bytes
         dy = torch.nn.functional.pad(dy, (0, -N % 8))
-    return _int8_wgrad(_dense(dy), _dense(q), s.contiguous())[:N]
+    dy, q, s = _dense(dy), _dense(q), s.contiguous()
+    dw = _wgrad(dy, q, s) if _plain(dy, q, s) else _int8_wgrad(dy, q, s)
+    return dw if dw.shape[0] == N else dw[:N]

@@ -15,8 +15,8 @@ from __future__ import annotations
 
 import torch
 
-from .._lib import call, workspace
-from .common import HALF_TYPES, _check_half, _check_same_device, _check_vec, _dense, _stream
+from .._lib import workspace
+from .common import HALF_TYPES, _check_half, _check_same_device, _check_vec, _dense, _launch, _plain
 
 __all__ = ["sandwich_norm", "sandwich_norm_bwd", "sandwich_norm_int8"]
 
@@ -27,18 +27,82 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# ------------------------------------------------------------------ launches --
+def _fwd(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps):
+    B, S, D = x.shape
+    h, z = torch.empty_like(x), torch.empty_like(x)
+    _launch("afb_sandwich_norm", x, x.data_ptr(), residual.data_ptr(), _ptr(gate), post_weight.data_ptr(),
+            pre_weight.data_ptr(), _ptr(shift), _ptr(scale), h.data_ptr(), z.data_ptr(), B, S, D,
+            residual_scale, eps, HALF_TYPES[x.dtype])
+    return h, z
+
+
+def _fwd_int8(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps):
+    B, S, D = x.shape
+    z = torch.empty_like(x)
+    q, s = torch.empty_like(x, dtype=torch.int8), x.new_empty((B * S, 1), dtype=F32)
+    _launch("afb_sandwich_norm_int8", x, x.data_ptr(), residual.data_ptr(), _ptr(gate), post_weight.data_ptr(),
+            pre_weight.data_ptr(), _ptr(shift), _ptr(scale), q.data_ptr(), s.data_ptr(), z.data_ptr(), B, S, D,
+            residual_scale, eps, HALF_TYPES[x.dtype])
+    return q, s, z
+
+
+def _bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale, residual_scale, eps):
+    B, S, D = z.shape
+    dx, dres = torch.empty_like(x), torch.empty_like(z)
+    dgate, dshift, dscale = (z.new_empty((B, D)) for _ in range(3))
+    dpost, dpre = torch.empty_like(post_weight), torch.empty_like(pre_weight)
+    if z.numel() == 0:
+        for t in (dgate, dshift, dscale, dpost, dpre):
+            t.zero_()
+        return dx, dres, dgate, dpost, dpre, dshift, dscale
+    ws, nbytes = workspace("afb_sandwich_norm_bwd", z.device, B, S, D)
+    _launch("afb_sandwich_norm_bwd", z, gh.data_ptr(), _ptr(gz), z.data_ptr(), x.data_ptr(), _ptr(gate),
+            post_weight.data_ptr(), pre_weight.data_ptr(), _ptr(scale), dx.data_ptr(), dres.data_ptr(),
+            dgate.data_ptr(), dpost.data_ptr(), dpre.data_ptr(), dshift.data_ptr(), dscale.data_ptr(),
+            B, S, D, residual_scale, eps, HALF_TYPES[z.dtype], ws.data_ptr(), nbytes)
+    return dx, dres, dgate, dpost, dpre, dshift, dscale
+
+
+def _saved(ctx, x, gate, post_weight, pre_weight, shift, scale, z, residual_scale, eps):
+    ctx.save_for_backward(x, gate, post_weight, pre_weight, scale, z)
+    ctx.has_shift = shift is not None
+    ctx.residual_scale = residual_scale
+    ctx.eps = eps
+
+
+def _grads(ctx, bwd, gh, gz):
+    x, gate, post_weight, pre_weight, scale, z = ctx.saved_tensors
+    dx, dres, dgate, dpost, dpre, dshift, dscale = bwd(
+        _dense(gh), None if gz is None else _dense(gz), z, x, gate, post_weight, pre_weight, scale,
+        ctx.residual_scale, ctx.eps)
+    return (dx, dres, dgate if gate is not None else None, dpost, dpre, dshift if ctx.has_shift else None,
+            dscale if scale is not None else None, None, None)
+
+
+class _SandwichFn(torch.autograd.Function):
+    """sandwich_norm's gradient where the launches are called directly."""
+
+    @staticmethod
+    def forward(ctx, x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps):
+        h, z = _fwd(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
+        _saved(ctx, x, gate, post_weight, pre_weight, shift, scale, z, residual_scale, eps)
+        return h, z
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gh, gz):
+        return _grads(ctx, _bwd, gh, gz)
+
+
+# ----------------------------------------------------------------- custom ops --
 @torch.library.custom_op("anima_flat_b200::sandwich_norm", mutates_args=())
 def _sandwich_norm(
     x: torch.Tensor, residual: torch.Tensor, gate: torch.Tensor | None, post_weight: torch.Tensor,
     pre_weight: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None,
     residual_scale: float, eps: float,
 ) -> tuple[torch.Tensor, torch.Tensor]:
-    B, S, D = x.shape
-    h, z = torch.empty_like(x), torch.empty_like(x)
-    call("afb_sandwich_norm", x.data_ptr(), residual.data_ptr(), _ptr(gate), post_weight.data_ptr(),
-         pre_weight.data_ptr(), _ptr(shift), _ptr(scale), h.data_ptr(), z.data_ptr(), B, S, D,
-         residual_scale, eps, HALF_TYPES[x.dtype], _stream(x))
-    return h, z
+    return _fwd(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
 
 
 @_sandwich_norm.register_fake
@@ -52,14 +116,7 @@ def _sandwich_norm_int8(
     pre_weight: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None,
     residual_scale: float, eps: float,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    B, S, D = x.shape
-    z = torch.empty_like(x)
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    s = torch.empty((B * S, 1), dtype=F32, device=x.device)
-    call("afb_sandwich_norm_int8", x.data_ptr(), residual.data_ptr(), _ptr(gate), post_weight.data_ptr(),
-         pre_weight.data_ptr(), _ptr(shift), _ptr(scale), q.data_ptr(), s.data_ptr(), z.data_ptr(), B, S, D,
-         residual_scale, eps, HALF_TYPES[x.dtype], _stream(x))
-    return q, s, z
+    return _fwd_int8(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
 
 
 @_sandwich_norm_int8.register_fake
@@ -74,20 +131,7 @@ def _sandwich_norm_bwd(
     post_weight: torch.Tensor, pre_weight: torch.Tensor, scale: torch.Tensor | None,
     residual_scale: float, eps: float,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    B, S, D = z.shape
-    dx, dres = torch.empty_like(x), torch.empty_like(z)
-    dgate, dshift, dscale = (torch.empty((B, D), dtype=z.dtype, device=z.device) for _ in range(3))
-    dpost, dpre = (torch.empty(D, dtype=F32, device=z.device) for _ in range(2))
-    if z.numel() == 0:
-        for t in (dgate, dshift, dscale, dpost, dpre):
-            t.zero_()
-        return dx, dres, dgate, dpost, dpre, dshift, dscale
-    ws, nbytes = workspace("afb_sandwich_norm_bwd", z.device, B, S, D)
-    call("afb_sandwich_norm_bwd", gh.data_ptr(), _ptr(gz), z.data_ptr(), x.data_ptr(), _ptr(gate),
-         post_weight.data_ptr(), pre_weight.data_ptr(), _ptr(scale), dx.data_ptr(), dres.data_ptr(),
-         dgate.data_ptr(), dpost.data_ptr(), dpre.data_ptr(), dshift.data_ptr(), dscale.data_ptr(),
-         B, S, D, residual_scale, eps, HALF_TYPES[z.dtype], ws.data_ptr(), nbytes, _stream(z))
-    return dx, dres, dgate, dpost, dpre, dshift, dscale
+    return _bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale, residual_scale, eps)
 
 
 @_sandwich_norm_bwd.register_fake
@@ -100,58 +144,56 @@ def _(gh, gz, z, x, gate, post_weight, pre_weight, scale, residual_scale, eps):
 
 def _setup(ctx, inputs, output):
     x, _, gate, post_weight, pre_weight, shift, scale, residual_scale, eps = inputs
-    ctx.save_for_backward(x, gate, post_weight, pre_weight, scale, output[1])
-    ctx.has_shift = shift is not None
-    ctx.residual_scale = residual_scale
-    ctx.eps = eps
+    _saved(ctx, x, gate, post_weight, pre_weight, shift, scale, output[1], residual_scale, eps)
 
 
 def _backward(ctx, gh, gz):
-    x, gate, post_weight, pre_weight, scale, z = ctx.saved_tensors
-    dx, dres, dgate, dpost, dpre, dshift, dscale = _sandwich_norm_bwd(
-        _dense(gh), None if gz is None else _dense(gz), z, x, gate, post_weight, pre_weight, scale,
-        ctx.residual_scale, ctx.eps)
-    return (dx, dres, dgate if gate is not None else None, dpost, dpre, dshift if ctx.has_shift else None,
-            dscale if scale is not None else None, None, None)
+    return _grads(ctx, _sandwich_norm_bwd, gh, gz)
 
 
 torch.library.register_autograd("anima_flat_b200::sandwich_norm", _backward, setup_context=_setup)
 
 
+# --------------------------------------------------------------------- public --
 def _weight(w: torch.Tensor, D: int, name: str) -> torch.Tensor:
+    if w.dtype is F32 and w.shape == (D,):
+        return _dense(w)
     if w.numel() != D:
         raise ValueError(f"{name} must be [{D}], got {list(w.shape)}")
     return _dense(w.to(F32).reshape(D))
 
 
-def _vec(v: torch.Tensor | None, x: torch.Tensor, name: str) -> torch.Tensor | None:
+def _vec(v: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype, name: str) -> torch.Tensor | None:
     if v is None:
         return None
-    if v.dtype != x.dtype:
-        raise ValueError(f"{name} must be {x.dtype}, got {v.dtype}")
-    _check_vec(v, x.shape[0], x.shape[2], name)
-    return _dense(v.reshape(x.shape[0], x.shape[2]))
+    if v.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype}, got {v.dtype}")
+    if v.shape == shape:
+        return _dense(v)
+    _check_vec(v, *shape, name)
+    return _dense(v.reshape(shape))
 
 
-def _check_rows(x: torch.Tensor, *like: tuple[str, torch.Tensor | None]) -> None:
+def _check_rows(x: torch.Tensor, *like: tuple[str, torch.Tensor | None]) -> tuple[int, int]:
     _check_half("activations", x)
-    if x.ndim != 3:
-        raise ValueError(f"expected [B, S, D] activations, got {list(x.shape)}")
-    D = x.shape[2]
+    shape = x.shape
+    if len(shape) != 3:
+        raise ValueError(f"expected [B, S, D] activations, got {list(shape)}")
+    D = shape[2]
     if D < 8 or D % 8 or D > 4096:
         raise ValueError(f"D must be a multiple of 8 in [8, 4096], got {D}")
     for name, t in like:
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError(f"{name} must be {x.dtype} {list(x.shape)}, got {t.dtype} {list(t.shape)}")
+        if t is not None and (t.shape != shape or t.dtype is not x.dtype):
+            raise ValueError(f"{name} must be {x.dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return shape[0], D
 
 
 def _args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps):
     _check_same_device(x, residual, gate, post_weight, pre_weight, shift, scale)
-    _check_rows(x, ("residual", residual))
-    D = x.shape[2]
-    return (_dense(x), _dense(residual), _vec(gate, x, "gate"), _weight(post_weight, D, "post_weight"),
-            _weight(pre_weight, D, "pre_weight"), _vec(shift, x, "shift"), _vec(scale, x, "scale"),
-            float(residual_scale), float(eps))
+    vec, dtype = _check_rows(x, ("residual", residual)), x.dtype
+    return (_dense(x), _dense(residual), _vec(gate, vec, dtype, "gate"), _weight(post_weight, vec[1], "post_weight"),
+            _weight(pre_weight, vec[1], "pre_weight"), _vec(shift, vec, dtype, "shift"),
+            _vec(scale, vec, dtype, "scale"), float(residual_scale), float(eps))
 
 
 def sandwich_norm(x, residual, gate, post_weight, pre_weight, shift=None, scale=None, residual_scale=1.0, eps=1e-6):
@@ -176,7 +218,12 @@ def sandwich_norm(x, residual, gate, post_weight, pre_weight, shift=None, scale=
     Raises:
         ValueError: On tensors off CUDA or unsupported dtypes or shapes.
     """
-    return _sandwich_norm(*_args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps))
+    args = _args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
+    if not _plain(*args[:7]):
+        return _sandwich_norm(*args)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:7]):
+        return _SandwichFn.apply(*args)
+    return _fwd(*args)
 
 
 def sandwich_norm_int8(x, residual, gate, post_weight, pre_weight, shift=None, scale=None, residual_scale=1.0,
@@ -193,7 +240,8 @@ def sandwich_norm_int8(x, residual, gate, post_weight, pre_weight, shift=None, s
     Raises:
         ValueError: On tensors off CUDA or unsupported dtypes or shapes.
     """
-    return _sandwich_norm_int8(*_args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps))
+    args = _args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
+    return (_fwd_int8 if _plain(*args[:7]) else _sandwich_norm_int8)(*args)
 
 
 def sandwich_norm_bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale=None, residual_scale=1.0, eps=1e-6):
@@ -217,9 +265,8 @@ def sandwich_norm_bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale=None, r
         ValueError: On tensors off CUDA or unsupported dtypes or shapes.
     """
     _check_same_device(gh, gz, z, x, gate, post_weight, pre_weight, scale)
-    _check_rows(z, ("x", x), ("gh", gh), ("gz", gz))
-    D = z.shape[2]
-    return _sandwich_norm_bwd(
-        _dense(gh), None if gz is None else _dense(gz), _dense(z), _dense(x), _vec(gate, z, "gate"),
-        _weight(post_weight, D, "post_weight"), _weight(pre_weight, D, "pre_weight"), _vec(scale, z, "scale"),
-        float(residual_scale), float(eps))
+    vec, dtype = _check_rows(z, ("x", x), ("gh", gh), ("gz", gz)), z.dtype
+    args = (_dense(gh), None if gz is None else _dense(gz), _dense(z), _dense(x), _vec(gate, vec, dtype, "gate"),
+            _weight(post_weight, vec[1], "post_weight"), _weight(pre_weight, vec[1], "pre_weight"),
+            _vec(scale, vec, dtype, "scale"), float(residual_scale), float(eps))
+    return (_bwd if _plain(*args[:8]) else _sandwich_norm_bwd)(*args)

@@ -300,6 +300,13 @@ int afb_int8_restore(const void* q, const void* s, void* y, int64_t rows, int64_
 int afb_int8_linear(const void* q, const void* s, const void* w, const void* v, const void* bias,
                     void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream);
 
+/* The same from x [M, K] of `dtype`, or x * cols where cols [K] fp32 is not
+ * NULL, quantised as by afb_rowquant_int8; v may be NULL (1).  K at most
+ * 16384.  Workspace: M * (K + 4) bytes, 16-byte aligned, overwritten. */
+int afb_int8_linear_x(const void* x, const void* cols, const void* w, const void* v,
+                      const void* bias, void* y, int64_t M, int64_t N, int64_t K, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* dw[n, k] = sum_t dy[t, n] q[t, k] s[t], summed in fp32.  dy [rows, N], N a
  * multiple of 8; q [rows, K], K a multiple of 16; s [rows]; dw [N, K] of
  * `dtype` (zero where rows = 0). */
