@@ -41,6 +41,65 @@ __device__ __forceinline__ float scaled(uint32_t acc, float s, float v, float b)
   return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(acc)), s), v), b);
 }
 
+// Writes the warp's 32 channels from `run` and `cols` tokens from m0 of an
+// accumulator at `acc`.  sm: the tokens' scales; vn, b: scale and bias of the
+// lane's channel; st0: two pieces of 1024 bytes of the warp's own.
+template <int DT>
+__device__ __forceinline__ void emit(const LinearArgs& a, uint32_t acc, const float* sm, uint32_t st0, int run, int m0,
+                                     int cols, float vn, float b) {
+  const int lane = threadIdx.x & 31;
+  // 16 tokens at a time: fragments of 8 channels x 8 tokens, scaled and
+  // rounded, are transposed into rows of 32 channels, which leave as
+  // whole 64-byte runs.  16-byte chunks of the rows are swizzled, so
+  // that neither side meets a bank twice.
+  float vf[4], bf[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    vf[g] = __shfl_sync(kFull, vn, (lane >> 2) + 8 * g);
+    bf[g] = __shfl_sync(kFull, b, (lane >> 2) + 8 * g);
+  }
+  const bool wide = a.N % 8 == 0;
+#pragma unroll 2
+  for (int c = 0; c < cols; c += 16) {
+    const uint32_t stage = st0 + ((c >> 4) & 1) * 1024;
+    uint32_t v[2][8];
+    tmem_ld_frag2(acc + c, v[0]);
+    tmem_ld_frag2(acc + (16u << 16) + c, v[1]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 s2 = *reinterpret_cast<const float2*>(&sm[c + 8 * i + 2 * (lane & 3)]);
+      uint32_t o[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t* p = &v[g >> 1][4 * i + 2 * (g & 1)];
+        o[g] = pack2<DT>(scaled(p[0], s2.x, vf[g], bf[g]), scaled(p[1], s2.y, vf[g], bf[g]));
+      }
+      const int tok = 8 * i + (lane & 7);
+      stmatrix_trans(stage + tok * 64 + (((lane >> 3) ^ (tok >> 1)) & 3) * 16, o);
+    }
+    __syncwarp();
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int tok = 8 * i + (lane >> 2), at = run + (lane & 3) * 8;
+        const uint4 w = lds16a(stage + tok * 64 + (((lane & 3) ^ (tok >> 1)) & 3) * 16);
+        if (c + tok < cols && at < a.N) st16(a.y + static_cast<int64_t>(m0 + c + tok) * a.N + at, w);
+      }
+    } else {
+#pragma unroll 4
+      for (int tok = 0; tok < 16; ++tok) {
+        uint16_t w;
+        asm volatile("ld.shared.u16 %0, [%1];"
+                     : "=h"(w)
+                     : "r"(stage + tok * 64 + (((lane >> 3) ^ (tok >> 1)) & 3) * 16 + (lane & 7) * 2)
+                     : "memory");
+        if (c + tok < cols && run + lane < a.N) a.y[static_cast<int64_t>(m0 + c + tok) * a.N + run + lane] = w;
+      }
+    }
+  }
+}
+
 template <int BN, int DT>
 __global__ void __launch_bounds__(kThreads, BN < 256 ? 2 : 1)
 int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap,
@@ -157,58 +216,7 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
       tc_fence_after();
       const int cols = min(BN, a.M - m0);
       if (split == 1) {
-        // 16 tokens at a time: fragments of 8 channels x 8 tokens, scaled and
-        // rounded, are transposed into rows of 32 channels, which leave as
-        // whole 64-byte runs.  16-byte chunks of the rows are swizzled, so
-        // that neither side meets a bank twice.
-        float vf[4], bf[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          vf[g] = __shfl_sync(kFull, vn, (lane >> 2) + 8 * g);
-          bf[g] = __shfl_sync(kFull, b, (lane >> 2) + 8 * g);
-        }
-        const uint32_t st0 = smem_addr(out[warp - 2][0]);
-        const int run = n0 + quad * 32;
-        const bool wide = a.N % 8 == 0;
-#pragma unroll 2
-        for (int c = 0; c < cols; c += 16) {
-          const uint32_t stage = st0 + ((c >> 4) & 1) * 1024;
-          uint32_t v[2][8];
-          tmem_ld_frag2(trow + buf * BN + c, v[0]);
-          tmem_ld_frag2(trow + (16u << 16) + buf * BN + c, v[1]);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float2 s2 = *reinterpret_cast<const float2*>(&sm[buf][c + 8 * i + 2 * (lane & 3)]);
-            uint32_t o[4];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const uint32_t* p = &v[g >> 1][4 * i + 2 * (g & 1)];
-              o[g] = pack2<DT>(scaled(p[0], s2.x, vf[g], bf[g]), scaled(p[1], s2.y, vf[g], bf[g]));
-            }
-            const int tok = 8 * i + (lane & 7);
-            stmatrix_trans(stage + tok * 64 + (((lane >> 3) ^ (tok >> 1)) & 3) * 16, o);
-          }
-          __syncwarp();
-          if (wide) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int tok = 8 * i + (lane >> 2), at = run + (lane & 3) * 8;
-              const uint4 w = lds16a(stage + tok * 64 + (((lane & 3) ^ (tok >> 1)) & 3) * 16);
-              if (c + tok < cols && at < a.N) st16(a.y + static_cast<int64_t>(m0 + c + tok) * a.N + at, w);
-            }
-          } else {
-#pragma unroll 4
-            for (int tok = 0; tok < 16; ++tok) {
-              uint16_t w;
-              asm volatile("ld.shared.u16 %0, [%1];"
-                           : "=h"(w)
-                           : "r"(stage + tok * 64 + (((lane >> 3) ^ (tok >> 1)) & 3) * 16 + (lane & 7) * 2)
-                           : "memory");
-              if (c + tok < cols && nok) a.y[static_cast<int64_t>(m0 + c + tok) * a.N + ch] = w;
-            }
-          }
-        }
+        emit<DT>(a, trow + buf * BN, sm[buf], smem_addr(out[warp - 2][0]), n0 + quad * 32, m0, cols, vn, b);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(acce + 8 * buf);
@@ -276,6 +284,159 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
   }
 }
 
+// The same for large products, by pairs of CTAs: a tile is 256 channels by BN
+// tokens, a CTA brings and emits its 128 channels and brings half of the
+// tokens, the first CTA issues the matrix instructions for both.  A stage then
+// costs a CTA (128 + BN / 2) rows from L2 for the work of 128 x BN: alone, with
+// 256 tokens, it asks for 96 bytes a clock, more than L2 gives.
+__host__ __device__ constexpr int pair_stage_bytes(int bn) { return (kTileN + bn / 2) * kKBlock; }
+__host__ __device__ constexpr int pair_stages(int bn) { return bn >= 256 ? 6 : 8; }
+__host__ __device__ constexpr int pair_smem(int bn) { return pair_stages(bn) * pair_stage_bytes(bn) + 1024; }
+
+template <int BN, int DT>
+__global__ void __launch_bounds__(kThreads, 1)
+int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap,
+                        const LinearArgs a) {
+  constexpr int ST = pair_stages(BN), SB = pair_stage_bytes(BN);
+  extern __shared__ uint8_t dyn[];
+  __shared__ __align__(8) uint64_t bars[2 * ST + 4];
+  __shared__ __align__(8) float sm[2][BN];
+  __shared__ __align__(128) uint8_t out[4][2][1024];
+  __shared__ uint32_t tslot;
+  const uint32_t ring = (smem_addr(dyn) + 1023) & ~1023u;
+  const uint32_t full = smem_addr(bars), empty = full + 8 * ST, accf = empty + 8 * ST, acce = accf + 16;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_rank());
+  if (threadIdx.x == 0) {
+    prefetch_map(&wmap);
+    prefetch_map(&qmap);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(accf + 8 * i, 1);
+      mbar_init(acce + 8 * i, 8);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_pair(smem_addr(&tslot), lin_tmem(BN));
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tslot;
+  pdl_wait();
+  pdl_trigger();
+
+  const int blocks = (a.K + kKBlock - 1) / kKBlock;
+  const int first = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
+  auto channel0 = [&](int tile) { return (tile % a.ntiles) * 2 * kTileN + rank * kTileN; };
+
+  if (warp == 0) {
+    const uint32_t full0 = peer_addr(full, 0);
+    int it = 0, sent = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < a.tiles; tile += step) {
+      const int n0 = channel0(tile), m0 = (tile / a.ntiles) * BN + rank * (BN / 2);
+      for (int kb = 0; kb < blocks; ++kb, ++it) {
+        const int st = it % ST;
+        if (it >= ST && !mbar_wait(empty + 8 * st, ((it / ST) - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(full + 8 * st, 2 * SB);
+          tma_load_pair(ring + st * SB, &wmap, kb * kKBlock, n0, full0 + 8 * st);
+          tma_load_pair(ring + st * SB + kTileN * kKBlock, &qmap, kb * kKBlock, m0, full0 + 8 * st);
+        }
+        __syncwarp();
+        sent = it + 1;
+      }
+    }
+    // After a wait that gave up: the first CTA's barriers count both CTAs'
+    // copies, and neither leaves before the cluster's last barrier.
+    if (!ok && rank == 0)
+      for (int i = sent > ST ? sent - ST : 0; i < sent; ++i) mbar_wait(full + 8 * (i % ST), (i / ST) & 1);
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc =
+          (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(2 * kTileN >> 4) << 24);
+      const uint64_t desc0 = smem_desc(ring, 16, 1024);
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < a.tiles; tile += step, ++n) {
+        const int buf = n & 1;
+        if (n >= 2 && !mbar_wait(acce + 8 * buf, ((n >> 1) - 1) & 1)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
+          const int st = it % ST;
+          if (!mbar_wait(full + 8 * st, (it / ST) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t da = desc0 + static_cast<uint64_t>(st * (SB >> 4));
+            const uint64_t db = da + (kTileN * kKBlock >> 4);
+#pragma unroll
+            for (int k = 0; k < kKBlock / 32; ++k)
+              mma_i8_pair(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, kb > 0 || k > 0);
+            mma_commit_pair(empty + 8 * st);
+          }
+          __syncwarp();
+        }
+        if (elect_one()) mma_commit_pair(accf + 8 * buf);
+        __syncwarp();
+      }
+    }
+  } else {
+    const int quad = warp & 3;
+    const int et = static_cast<int>(threadIdx.x) - 64;
+    const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t acce0 = peer_addr(acce, 0);
+    int n = 0;
+    bool ok = true;
+    for (int tile = first; tile < a.tiles; tile += step, ++n) {
+      const int buf = n & 1;
+      const int n0 = channel0(tile), m0 = (tile / a.ntiles) * BN;
+      const int ch = n0 + quad * 32 + lane;
+      const float vn = ch < a.N ? scale_of(a, ch) : 0.0f;
+      const float b = ch < a.N && a.bias != nullptr ? load1<DT>(a.bias + ch) : 0.0f;
+      for (int i = et; i < BN; i += 128) sm[buf][i] = m0 + i < a.M ? __ldg(a.s + m0 + i) : 0.0f;
+      named_bar_sync(1, 128);
+      ok = ok && mbar_wait(accf + 8 * buf, (n >> 1) & 1);
+      if (!ok) continue;
+      tc_fence_after();
+      emit<DT>(a, trow + buf * BN, sm[buf], smem_addr(out[warp - 2][0]), n0 + quad * 32, m0, min(BN, a.M - m0), vn, b);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(acce0 + 8 * buf);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free_pair(tmem, lin_tmem(BN));
+  }
+}
+
+template <int BN, int DT>
+static cudaError_t launch_pair(const void* q, const void* w, LinearArgs a, cudaStream_t st) {
+  CUtensorMap wmap, qmap;
+  const uint64_t K = static_cast<uint64_t>(a.K);
+  cudaError_t e = make_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w, K, a.N, K, kKBlock, kTileN);
+  if (e == cudaSuccess)
+    e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, q, K, a.M, K, kKBlock, BN / 2);
+  if (e == cudaSuccess) e = ensure_smem(int8_linear_pair_kernel<BN, DT>, pair_smem(BN));
+  if (e != cudaSuccess) return e;
+  a.ntiles = (a.N + 2 * kTileN - 1) / (2 * kTileN);
+  a.tiles = a.ntiles * ((a.M + BN - 1) / BN);
+  const int grid = 2 * std::min(a.tiles, device_info().sms / 2);
+  return launch_cluster(int8_linear_pair_kernel<BN, DT>, dim3(grid), dim3(kThreads), pair_smem(BN), 2, st, wmap, qmap, a);
+}
+
 template <int BN, int DT>
 static cudaError_t launch_linear(const void* q, const void* w, LinearArgs a, int split, cudaStream_t st) {
   CUtensorMap wmap, qmap;
@@ -313,12 +474,12 @@ static cudaError_t linear(const void* q, const void* w, const LinearArgs& a, cud
   if (d.error != cudaSuccess) return d.error;
   int bn, split;
   linear_shape(a.M, a.N, a.K, d.sms, &bn, &split);
+  if (bn == 256) return launch_pair<256, DT>(q, w, a, st);
   switch (bn) {
     case 16: return launch_linear<16, DT>(q, w, a, split, st);
     case 32: return launch_linear<32, DT>(q, w, a, split, st);
     case 64: return launch_linear<64, DT>(q, w, a, split, st);
-    case 128: return launch_linear<128, DT>(q, w, a, split, st);
-    default: return launch_linear<256, DT>(q, w, a, split, st);
+    default: return launch_linear<128, DT>(q, w, a, split, st);
   }
 }
 
