@@ -41,63 +41,24 @@ __device__ __forceinline__ float scaled(uint32_t acc, float s, float v, float b)
   return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(acc)), s), v), b);
 }
 
-// Writes the warp's 32 channels from `run` and `cols` tokens from m0 of an
-// accumulator at `acc`.  sm: the tokens' scales; vn, b: scale and bias of the
-// lane's channel; st0: two pieces of 1024 bytes of the warp's own.
+// The warp's 32 channels from `run` and `cols` tokens from m0 of an accumulator
+// at `acc`, scaled.  sm: the tokens' scales; vn, b: scale and bias of the
+// lane's channel.
 template <int DT>
 __device__ __forceinline__ void emit(const LinearArgs& a, uint32_t acc, const float* sm, uint32_t st0, int run, int m0,
                                      int cols, float vn, float b) {
   const int lane = threadIdx.x & 31;
-  // 16 tokens at a time: fragments of 8 channels x 8 tokens, scaled and
-  // rounded, are transposed into rows of 32 channels, which leave as
-  // whole 64-byte runs.  16-byte chunks of the rows are swizzled, so
-  // that neither side meets a bank twice.
   float vf[4], bf[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     vf[g] = __shfl_sync(kFull, vn, (lane >> 2) + 8 * g);
     bf[g] = __shfl_sync(kFull, b, (lane >> 2) + 8 * g);
   }
-  const bool wide = a.N % 8 == 0;
-#pragma unroll 2
-  for (int c = 0; c < cols; c += 16) {
-    const uint32_t stage = st0 + ((c >> 4) & 1) * 1024;
-    uint32_t v[2][8];
-    tmem_ld_frag2(acc + c, v[0]);
-    tmem_ld_frag2(acc + (16u << 16) + c, v[1]);
-    tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float2 s2 = *reinterpret_cast<const float2*>(&sm[c + 8 * i + 2 * (lane & 3)]);
-      uint32_t o[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint32_t* p = &v[g >> 1][4 * i + 2 * (g & 1)];
-        o[g] = pack2<DT>(scaled(p[0], s2.x, vf[g], bf[g]), scaled(p[1], s2.y, vf[g], bf[g]));
-      }
-      const int tok = 8 * i + (lane & 7);
-      stmatrix_trans(stage + tok * 64 + (((lane >> 3) ^ (tok >> 1)) & 3) * 16, o);
-    }
-    __syncwarp();
-    if (wide) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int tok = 8 * i + (lane >> 2), at = run + (lane & 3) * 8;
-        const uint4 w = lds16a(stage + tok * 64 + (((lane & 3) ^ (tok >> 1)) & 3) * 16);
-        if (c + tok < cols && at < a.N) st16(a.y + static_cast<int64_t>(m0 + c + tok) * a.N + at, w);
-      }
-    } else {
-#pragma unroll 4
-      for (int tok = 0; tok < 16; ++tok) {
-        uint16_t w;
-        asm volatile("ld.shared.u16 %0, [%1];"
-                     : "=h"(w)
-                     : "r"(stage + tok * 64 + (((lane >> 3) ^ (tok >> 1)) & 3) * 16 + (lane & 7) * 2)
-                     : "memory");
-        if (c + tok < cols && run + lane < a.N) a.y[static_cast<int64_t>(m0 + c + tok) * a.N + run + lane] = w;
-      }
-    }
-  }
+  emit_columns(acc, st0, cols, a.y + static_cast<int64_t>(m0) * a.N, a.N, run,
+               [&](int c, int g, uint32_t lo, uint32_t hi) {
+                 const float2 s2 = *reinterpret_cast<const float2*>(&sm[c]);
+                 return pack2<DT>(scaled(lo, s2.x, vf[g], bf[g]), scaled(hi, s2.y, vf[g], bf[g]));
+               });
 }
 
 template <int BN, int DT>
@@ -366,11 +327,11 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
       bool ok = true;
       for (int tile = first; ok && tile < a.tiles; tile += step, ++n) {
         const int buf = n & 1;
-        if (n >= 2 && !mbar_wait(acce + 8 * buf, ((n >> 1) - 1) & 1)) break;
+        if (n >= 2 && !mbar_wait_cluster(acce + 8 * buf, ((n >> 1) - 1) & 1)) break;
         tc_fence_after();
         for (int kb = 0; kb < blocks; ++kb, ++it) {
           const int st = it % ST;
-          if (!mbar_wait(full + 8 * st, (it / ST) & 1)) {
+          if (!mbar_wait_cluster(full + 8 * st, (it / ST) & 1)) {
             ok = false;
             break;
           }

@@ -65,6 +65,18 @@ __device__ __forceinline__ void convert16(const uint4 q, float s, uint4& lo, uin
   hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
+// A token's 16 channels 16 part .. of a stage, converted, to the operand at
+// `dst`: chunk of 64 channels, row of the token, 16-byte pieces swizzled by it.
+template <int DT>
+__device__ __forceinline__ void put_converted(uint32_t dst, int t, int part, const uint4 code, float s) {
+  uint4 lo, hi;
+  convert16<DT>(code, s, lo, hi);
+  const uint32_t row = dst + (part >> 2) * (kTok * 128) + t * 128;
+  const uint32_t p0 = ((2 * (part & 3)) ^ (t & 7)) * 16;
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + p0), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (p0 ^ 16)), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+}
+
 template <int BN, int DT>
 __global__ void __launch_bounds__(wg_threads(BN), BN <= 64 ? 2 : 1)
 int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
@@ -177,13 +189,7 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
       for (int i = 0; i < 4; ++i) {
         const int t = i * 16 + w * 4 + (lane >> 3);
         const float sc = __shfl_sync(kFull, now, half + i * 4 + (lane >> 3));
-        uint4 lo, hi;
-        convert16<DT>(code[i], sc, lo, hi);
-        // chunk of 64 channels, row of the token, 16-byte pieces swizzled by the row
-        const uint32_t row = base + (part >> 2) * (kTok * 128) + t * 128;
-        const uint32_t p0 = ((2 * (part & 3)) ^ (t & 7)) * 16;
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + p0), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (p0 ^ 16)), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+        put_converted<DT>(base, t, part, code[i], sc);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -258,6 +264,232 @@ static cudaError_t launch_wgrad(const void* dy, const void* q, WgradArgs a, int 
                         gmap, a, split);
 }
 
+// The same for many columns, by pairs of CTAs: a tile is 256 channels by 256
+// columns, a CTA converts and emits its 128 channels and brings half of the
+// columns; the first CTA issues the matrix instructions for both.  Codes, dy
+// and converted stages have rings of their own: a stage's copies take about
+// 1500 cycles and its conversion 700, its matrix instructions 512, so codes are
+// asked for eight stages ahead, dy five, and four are converted at a time.
+constexpr int kPairCols = 256;
+constexpr int kQRing = 8, kDRing = 5, kCRing = 4;
+constexpr int kQBytes = kTok * kCh, kDBytes = kPairCols / 2 * kTok * 2, kCBytes = kCh * kTok * 2;
+constexpr int kPairSmem = kQRing * kQBytes + kDRing * kDBytes + kCRing * kCBytes + 1024;
+// Copies of dy, matrix instructions, copies of codes, one idle; four warps of
+// the epilogue; kCRing groups of four that convert.
+constexpr int kPairThreads = 128 + 128 + 128 * kCRing;
+
+template <int DT>
+__global__ void __launch_bounds__(kPairThreads, 1)
+int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
+                       const WgradArgs a, int tiles) {
+  // a group meets its stage of either ring in every phase
+  static_assert(kQRing % kCRing == 0, "");
+  constexpr int kBars = 2 * (kQRing + kDRing + kCRing) + 4;
+  extern __shared__ uint8_t dyn[];
+  __shared__ __align__(8) uint64_t bars[kBars];
+  __shared__ __align__(128) uint8_t out[4][2][1024];
+  __shared__ uint32_t tslot;
+  const uint32_t cring = (smem_addr(dyn) + 1023) & ~1023u;
+  const uint32_t dring = cring + kCRing * kCBytes, qring = dring + kDRing * kDBytes;
+  const uint32_t qfull = smem_addr(bars), qempty = qfull + 8 * kQRing, dfull = qempty + 8 * kQRing;
+  const uint32_t dempty = dfull + 8 * kDRing, cfull = dempty + 8 * kDRing, cempty = cfull + 8 * kCRing;
+  const uint32_t accf = cempty + 8 * kCRing, acce = accf + 16;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_rank());
+  if (threadIdx.x == 0) {
+    prefetch_map(&qmap);
+    prefetch_map(&gmap);
+    for (int i = 0; i < kQRing; ++i) {
+      mbar_init(qfull + 8 * i, 1);
+      mbar_init(qempty + 8 * i, 4);
+    }
+    for (int i = 0; i < kDRing; ++i) {
+      mbar_init(dfull + 8 * i, 1);
+      mbar_init(dempty + 8 * i, 1);
+    }
+    for (int i = 0; i < kCRing; ++i) {
+      mbar_init(cfull + 8 * i, 8);
+      mbar_init(cempty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(accf + 8 * i, 1);
+      mbar_init(acce + 8 * i, 8);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_pair(smem_addr(&tslot), 2 * kPairCols);
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tslot;
+  pdl_wait();
+  pdl_trigger();
+
+  const int blocks = (a.T + kTok - 1) / kTok;
+  const int first = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
+  const int mine = first < tiles ? (tiles - first + step - 1) / step : 0;
+  auto channel0 = [&](int tile) { return (tile % a.ktiles) * 2 * kCh + rank * kCh; };
+  auto column0 = [&](int tile) { return (tile / a.ktiles) * kPairCols; };
+
+  if (warp == 0) {
+    const uint32_t dfull0 = peer_addr(dfull, 0);
+    int it = 0, sent = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < tiles; tile += step) {
+      const int n0 = column0(tile) + rank * (kPairCols / 2);
+      for (int t = 0; t < blocks; ++t, ++it) {
+        const int st = it % kDRing;
+        if (it >= kDRing && !mbar_wait(dempty + 8 * st, ((it / kDRing) - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(dfull + 8 * st, 2 * kDBytes);
+#pragma unroll
+          for (int c = 0; c < kPairCols / 128; ++c)
+            tma_load_pair(dring + st * kDBytes + c * kTok * 128, &gmap, n0 + 64 * c, t * kTok, dfull0 + 8 * st);
+        }
+        __syncwarp();
+        sent = it + 1;
+      }
+    }
+    // After a wait that gave up: the first CTA's barriers count both CTAs'
+    // copies, and neither leaves before the cluster's last barrier.
+    if (!ok && rank == 0)
+      for (int i = sent > kDRing ? sent - kDRing : 0; i < sent; ++i) mbar_wait(dfull + 8 * (i % kDRing), (i / kDRing) & 1);
+  } else if (warp == 2) {
+    int it = 0, sent = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < tiles; tile += step) {
+      const int k0 = channel0(tile);
+      for (int t = 0; t < blocks; ++t, ++it) {
+        const int st = it % kQRing;
+        if (it >= kQRing && !mbar_wait(qempty + 8 * st, ((it / kQRing) - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(qfull + 8 * st, kQBytes);
+          tma_load(qring + st * kQBytes, &qmap, k0, t * kTok, qfull + 8 * st);
+        }
+        __syncwarp();
+        sent = it + 1;
+      }
+    }
+    if (!ok)
+      for (int i = sent > kQRing ? sent - kQRing : 0; i < sent; ++i) mbar_wait(qfull + 8 * (i % kQRing), (i / kQRing) & 1);
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t type = DT == kBf16 ? 1u : 0u;
+      constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) |
+                                 (uint32_t(kPairCols >> 3) << 17) | (uint32_t(2 * kCh >> 4) << 24);
+      const uint64_t ca = smem_desc(cring, kTok * 128, 1024), cb = smem_desc(dring, kTok * 128, 1024);
+      int it = 0;
+      bool ok = true;
+      for (int n = 0; ok && n < mine; ++n) {
+        const int buf = n & 1;
+        if (n >= 2 && !mbar_wait_cluster(acce + 8 * buf, ((n >> 1) - 1) & 1)) break;
+        tc_fence_after();
+        for (int t = 0; t < blocks; ++t, ++it) {
+          const int ds = it % kDRing, cs = it % kCRing;
+          if (!mbar_wait_cluster(dfull + 8 * ds, (it / kDRing) & 1) || !mbar_wait_cluster(cfull + 8 * cs, (it / kCRing) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t da = ca + static_cast<uint64_t>(cs * (kCBytes >> 4));
+            const uint64_t db = cb + static_cast<uint64_t>(ds * (kDBytes >> 4));
+#pragma unroll
+            for (int k = 0; k < kTok / 16; ++k)
+              mma_f16_pair(tmem + buf * kPairCols, da + k * (2048 >> 4), db + k * (2048 >> 4), idesc, t > 0 || k > 0);
+            mma_commit_pair(dempty + 8 * ds);
+            mma_commit_pair(cempty + 8 * cs);
+          }
+          __syncwarp();
+        }
+        if (elect_one()) mma_commit_pair(accf + 8 * buf);
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 8) {
+    // As in the kernel above: a warp converts 16 tokens of its group's stages.
+    const int w = warp & 3, g = (warp - 8) >> 2, part = lane & 7;
+    const int total = mine * blocks;
+    const uint32_t cfull0 = peer_addr(cfull, 0);
+    auto scale_at = [&](int it) {
+      const int at = it + (lane >> 4) * kCRing;
+      const int t = (at % blocks) * kTok + ((lane >> 2) & 3) * 16 + w * 4 + (lane & 3);
+      return at < total && t < a.T ? __ldg(a.s + t) : 0.0f;
+    };
+    float now = 0.0f, next = scale_at(g);
+    int half = 0;
+    for (int it = g; it < total; it += kCRing, half ^= 16) {
+      const int qs = it % kQRing;
+      const uint32_t dst = cring + g * kCBytes, src = qring + qs * kQBytes;
+      if (half == 0) {
+        now = next;
+        next = scale_at(it + 2 * kCRing);
+      }
+      if (!mbar_wait(qfull + 8 * qs, (it / kQRing) & 1)) break;
+      if (it >= kCRing && !mbar_wait(cempty + 8 * g, ((it / kCRing) - 1) & 1)) break;
+      uint4 code[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) code[i] = lds16a(src + (i * 16 + w * 4 + (lane >> 3)) * kCh + part * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = i * 16 + w * 4 + (lane >> 3);
+        const float sc = __shfl_sync(kFull, now, half + i * 4 + (lane >> 3));
+        put_converted<DT>(dst, t, part, code[i], sc);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(qempty + 8 * qs);
+        mbar_arrive_at(cfull0 + 8 * g);
+      }
+    }
+  } else if (warp >= 4) {
+    const int quad = warp & 3;
+    const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t acce0 = peer_addr(acce, 0);
+    int n = 0;
+    for (int tile = first; tile < tiles; tile += step, ++n) {
+      const int buf = n & 1, n0 = column0(tile);
+      if (!mbar_wait(accf + 8 * buf, (n >> 1) & 1)) break;
+      tc_fence_after();
+      emit_columns(trow + buf * kPairCols, smem_addr(out[quad][0]), min(kPairCols, a.N - n0),
+                   a.dw + static_cast<int64_t>(n0) * a.K, a.K, channel0(tile) + quad * 32,
+                   [](int, int, uint32_t lo, uint32_t hi) { return pack2<DT>(__uint_as_float(lo), __uint_as_float(hi)); });
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(acce0 + 8 * buf);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free_pair(tmem, 2 * kPairCols);
+  }
+}
+
+template <int DT>
+static cudaError_t launch_wgrad_pair(const void* dy, const void* q, WgradArgs a, cudaStream_t st) {
+  CUtensorMap qmap, gmap;
+  cudaError_t e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, q, a.K, a.T, a.K, kCh, kTok);
+  if (e == cudaSuccess)
+    e = make_map(&gmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B, dy, a.N, a.T,
+                 static_cast<uint64_t>(a.N) * 2, 64, kTok);
+  if (e == cudaSuccess) e = ensure_smem(int8_wgrad_pair_kernel<DT>, kPairSmem);
+  if (e != cudaSuccess) return e;
+  a.ktiles = (a.K + 2 * kCh - 1) / (2 * kCh);
+  const int tiles = a.ktiles * ((a.N + kPairCols - 1) / kPairCols);
+  const int grid = 2 * std::min(tiles, device_info().sms / 2);
+  return launch_cluster(int8_wgrad_pair_kernel<DT>, dim3(grid), dim3(kPairThreads), kPairSmem, 2, st, qmap, gmap, a, tiles);
+}
+
 // Columns of a tile and parts along the tokens: the narrowest tile that holds
 // all columns, up to 128, or 256 where that still gives every multiprocessor a
 // tile; what is left idle goes to parts of at least two stages.
@@ -279,12 +511,12 @@ static cudaError_t wgrad(const void* dy, const void* q, const WgradArgs& a, cuda
   if (d.error != cudaSuccess) return d.error;
   int bn, split;
   wgrad_shape(a.T, a.N, a.K, d.sms, &bn, &split);
+  if (bn == 256) return launch_wgrad_pair<DT>(dy, q, a, st);
   switch (bn) {
     case 16: return launch_wgrad<16, DT>(dy, q, a, split, st);
     case 32: return launch_wgrad<32, DT>(dy, q, a, split, st);
     case 64: return launch_wgrad<64, DT>(dy, q, a, split, st);
-    case 128: return launch_wgrad<128, DT>(dy, q, a, split, st);
-    default: return launch_wgrad<256, DT>(dy, q, a, split, st);
+    default: return launch_wgrad<128, DT>(dy, q, a, split, st);
   }
 }
 

@@ -134,9 +134,27 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
                "h"(static_cast<uint16_t>(3))
                : "memory");
 }
-// Arrives on a barrier of any CTA of the cluster.
+// mbar_wait for a barrier on which the cluster's other CTAs arrive.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kMaxWaitSpins; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  atomicOr(&g_afb_device_status, kStatusWaitTimeout);
+  return false;
+}
+// Arrives on a barrier of any CTA of the cluster.  What the arrival announces
+// (tensor memory read, or shared memory written and fenced for the matrix
+// unit) concerns this CTA's own units, so the default release is enough; one of
+// cluster scope waits for the thread's global stores and cost 1900 cycles here.
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Arrives on `bar` when the matrix instructions issued so far are done.
@@ -172,6 +190,61 @@ __device__ __forceinline__ uint4 lds16a(uint32_t addr) {
   return r;
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Writes `cols` columns of a warp's 32 accumulator lanes at `acc` as rows of a
+// row-major 16-bit matrix: column c, lane l goes to y[c * ld + run + l], where
+// run + l < ld.  value(c, g, lo, hi) gives the pair of columns c, c + 1 of lane
+// 8 g + t / 4 (t the thread's lane), rounded, from their 32 bits.
+//
+// 16 columns at a time: fragments of 8 lanes x 8 columns are transposed into
+// rows of 32 in the warp's own shared memory (st0: twice 1024 bytes, 128-byte
+// aligned), which leave as whole 64-byte runs.  The rows' 16-byte pieces are
+// swizzled, so that neither side meets a bank twice.  Lane by lane, in 2-byte
+// stores, the same took 1.8 times as long as the matrix instructions of a tile
+// with k = 2048.
+template <typename F>
+__device__ __forceinline__ void emit_columns(uint32_t acc, uint32_t st0, int cols, uint16_t* y, int ld, int run, F value) {
+  const int lane = threadIdx.x & 31;
+  const bool wide = ld % 8 == 0;
+#pragma unroll 2
+  for (int c = 0; c < cols; c += 16) {
+    const uint32_t stage = st0 + ((c >> 4) & 1) * 1024;
+    uint32_t v[2][8];
+    tmem_ld_frag2(acc + c, v[0]);
+    tmem_ld_frag2(acc + (16u << 16) + c, v[1]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t o[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t* p = &v[g >> 1][4 * i + 2 * (g & 1)];
+        o[g] = value(c + 8 * i + 2 * (lane & 3), g, p[0], p[1]);
+      }
+      const int row = 8 * i + (lane & 7);
+      stmatrix_trans(stage + row * 64 + (((lane >> 3) ^ (row >> 1)) & 3) * 16, o);
+    }
+    __syncwarp();
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 8 * i + (lane >> 2), at = run + (lane & 3) * 8;
+        const uint4 w = lds16a(stage + row * 64 + (((lane & 3) ^ (row >> 1)) & 3) * 16);
+        if (c + row < cols && at < ld) st16(y + static_cast<int64_t>(c + row) * ld + at, w);
+      }
+    } else {
+#pragma unroll 4
+      for (int row = 0; row < 16; ++row) {
+        uint16_t w;
+        asm volatile("ld.shared.u16 %0, [%1];"
+                     : "=h"(w)
+                     : "r"(stage + row * 64 + (((lane >> 3) ^ (row >> 1)) & 3) * 16 + (lane & 7) * 2)
+                     : "memory");
+        if (c + row < cols && run + lane < ld) y[static_cast<int64_t>(c + row) * ld + run + lane] = w;
+      }
+    }
+  }
+}
 
 // Clusters.
 __device__ __forceinline__ uint32_t cluster_rank() {
