@@ -30,18 +30,23 @@ struct WgradArgs {
 constexpr int kTok = 64;  // tokens of a stage
 constexpr int kCh = 128;  // channels of a tile
 
-// A stage: the converted operand, dy in chunks of 64 columns, the codes.
-__host__ __device__ constexpr int wg_chunks(int bn) { return bn < 64 ? 1 : bn / 64; }
+// A stage's copies (codes, and BN columns of dy in chunks of 64 at most) and
+// its converted operand have rings of their own, since copies take longest.
+// Two blocks share a multiprocessor up to 64 columns: with one, 120 blocks at
+// most run at once in clusters of eight.
+__host__ __device__ constexpr int wg_width(int bn) { return bn < 64 ? bn : 64; }  // columns of a chunk
+__host__ __device__ constexpr int wg_chunks(int bn) { return bn / wg_width(bn); }
+__host__ __device__ constexpr int wg_raw_bytes(int bn) { return kTok * kCh + bn * kTok * 2; }
 __host__ __device__ constexpr int wg_conv_bytes() { return kCh * kTok * 2; }
-__host__ __device__ constexpr int wg_stage_bytes(int bn) { return wg_conv_bytes() + wg_chunks(bn) * kTok * 128 + kTok * kCh; }
-__host__ __device__ constexpr int wg_stages(int bn) { return bn >= 128 ? 4 : 3; }
-// Groups of four warps that convert, one for each stage of the ring, and then
+__host__ __device__ constexpr int wg_raw(int bn) { return bn == 16 || bn >= 128 ? 6 : 3; }
+// Groups of four warps that convert, one for each converted stage, and then
 // write the results.  Sixteen warps on one stage after another took 0.58 us a
-// stage, the latency of one pass from wait to arrival.  A group meets its stage
-// in every phase: a wait by parity may be one phase behind its barrier, not two.
-__host__ __device__ constexpr int wg_groups(int bn) { return wg_stages(bn); }
-__host__ __device__ constexpr int wg_threads(int bn) { return 64 + 128 * wg_groups(bn); }
-__host__ __device__ constexpr int wg_smem(int bn) { return wg_stages(bn) * wg_stage_bytes(bn) + 1024; }
+// stage, the latency of one pass from wait to arrival.  A group meets its
+// stages of either ring in every phase: a wait by parity may be one phase
+// behind its barrier, not two.
+constexpr int kGroups = 3;
+constexpr int kWgThreads = 64 + 128 * kGroups;
+__host__ __device__ constexpr int wg_smem(int bn) { return kGroups * wg_conv_bytes() + wg_raw(bn) * wg_raw_bytes(bn) + 1024; }
 __host__ __device__ constexpr int wg_tmem(int bn) { return bn < 32 ? 32 : bn; }
 
 // Sixteen codes to two 16-byte pieces of the 16-bit type, times the scale.
@@ -78,24 +83,29 @@ __device__ __forceinline__ void put_converted(uint32_t dst, int t, int part, con
 }
 
 template <int BN, int DT>
-__global__ void __launch_bounds__(wg_threads(BN), BN <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(kWgThreads, BN <= 64 ? 2 : 1)
 int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
                   const WgradArgs a, int split) {
-  constexpr int ST = wg_stages(BN), SB = wg_stage_bytes(BN), CH = wg_chunks(BN), G = wg_groups(BN);
-  constexpr int kGOff = wg_conv_bytes(), kQOff = kGOff + CH * kTok * 128;
+  constexpr int R = wg_raw(BN), RB = wg_raw_bytes(BN), CB = wg_conv_bytes(), G = kGroups;
+  constexpr int kGOff = kTok * kCh, kRow = wg_width(BN) * 2;  // bytes of a chunk's row
+  static_assert(R % G == 0, "");
   extern __shared__ uint8_t dyn[];
-  __shared__ __align__(8) uint64_t bars[3 * ST + 1];
+  __shared__ __align__(8) uint64_t bars[2 * R + 2 * G + 1];
   __shared__ uint32_t tslot;
-  const uint32_t ring = (smem_addr(dyn) + 1023) & ~1023u;
-  const uint32_t full = smem_addr(bars), conv = full + 8 * ST, empty = conv + 8 * ST, accf = empty + 8 * ST;
+  const uint32_t ring = (smem_addr(dyn) + 1023) & ~1023u, raw = ring + G * CB;
+  const uint32_t full = smem_addr(bars), empty = full + 8 * R, conv = empty + 8 * R, cempty = conv + 8 * G;
+  const uint32_t accf = cempty + 8 * G;
   const int warp = warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     prefetch_map(&qmap);
     prefetch_map(&gmap);
-    for (int i = 0; i < ST; ++i) {
+    for (int i = 0; i < R; ++i) {
       mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 5);  // the converting warps, and the matrix instructions
+    }
+    for (int i = 0; i < G; ++i) {
       mbar_init(conv + 8 * i, 4);
-      mbar_init(empty + 8 * i, 1);
+      mbar_init(cempty + 8 * i, 1);
     }
     mbar_init(accf, 1);
     fence_mbar_init();
@@ -120,40 +130,42 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
     int sent = 0;
     bool ok = true;
     for (int it = 0; it < nb; ++it) {
-      const int st = it % ST;
-      const uint32_t base = ring + st * SB;
-      if (it >= ST && !mbar_wait(empty + 8 * st, ((it / ST) - 1) & 1)) {
+      const int st = it % R;
+      const uint32_t base = raw + st * RB;
+      if (it >= R && !mbar_wait(empty + 8 * st, ((it / R) - 1) & 1)) {
         ok = false;
         break;
       }
       if (elect_one()) {
-        mbar_arrive_expect_tx(full + 8 * st, SB - wg_conv_bytes());
-        tma_load(base + kQOff, &qmap, k0, (b0 + it) * kTok, full + 8 * st);
+        mbar_arrive_expect_tx(full + 8 * st, RB);
+        tma_load(base, &qmap, k0, (b0 + it) * kTok, full + 8 * st);
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-          tma_load(base + kGOff + c * kTok * 128, &gmap, n0 + 64 * c, (b0 + it) * kTok, full + 8 * st);
+        for (int c = 0; c < wg_chunks(BN); ++c)
+          tma_load(base + kGOff + c * kTok * kRow, &gmap, n0 + 64 * c, (b0 + it) * kTok, full + 8 * st);
       }
       __syncwarp();
       sent = it + 1;
     }
     if (!ok)  // copies still in flight land before the block ends
-      for (int i = sent > ST ? sent - ST : 0; i < sent; ++i) mbar_wait(full + 8 * (i % ST), (i / ST) & 1);
+      for (int i = sent > R ? sent - R : 0; i < sent; ++i) mbar_wait(full + 8 * (i % R), (i / R) & 1);
   } else if (warp == 1) {
     // fp32 sums; both operands 16-bit floats, outermost along k (bits 15, 16).
     constexpr uint32_t type = DT == kBf16 ? 1u : 0u;
     constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) |
                                (uint32_t(BN >> 3) << 17) | (uint32_t(kCh >> 4) << 24);
-    const uint64_t desc0 = smem_desc(ring, kTok * 128, 1024);
+    const uint64_t ca = smem_desc(ring, kTok * 128, 1024);
+    const uint64_t cb = smem_desc(raw + kGOff, kTok * kRow, 8 * kRow, kRow);
     for (int it = 0; it < nb; ++it) {
-      const int st = it % ST;
-      if (!mbar_wait(full + 8 * st, (it / ST) & 1) || !mbar_wait(conv + 8 * st, (it / ST) & 1)) break;
+      const int st = it % R, cs = it % G;
+      if (!mbar_wait(full + 8 * st, (it / R) & 1) || !mbar_wait(conv + 8 * cs, (it / G) & 1)) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t da = desc0 + static_cast<uint64_t>(st * (SB >> 4)), db = da + (kGOff >> 4);
+        const uint64_t da = ca + static_cast<uint64_t>(cs * (CB >> 4)), db = cb + static_cast<uint64_t>(st * (RB >> 4));
 #pragma unroll
-        for (int k = 0; k < kTok / 16; ++k)  // 16 tokens: two groups of 8 rows of 128 bytes
-          mma_f16(tmem, da + k * (2048 >> 4), db + k * (2048 >> 4), idesc, it > 0 || k > 0);
+        for (int k = 0; k < kTok / 16; ++k)  // 16 tokens: two groups of 8 rows
+          mma_f16(tmem, da + k * (2048 >> 4), db + k * (16 * kRow >> 4), idesc, it > 0 || k > 0);
         mma_commit(empty + 8 * st);
+        mma_commit(cempty + 8 * cs);
       }
       __syncwarp();
     }
@@ -171,29 +183,33 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
       return at < nb && t < a.T ? __ldg(a.s + t) : 0.0f;
     };
     const int g = (warp - 2) >> 2;
+    const uint32_t dst = ring + g * CB;
     float now = 0.0f, next = scale_at(g);
     int half = 0;
     for (int it = g; it < nb; it += G, half ^= 16) {
-      const int st = it % ST;
-      const uint32_t base = ring + st * SB;
+      const int st = it % R;
+      const uint32_t src = raw + st * RB;
       if (half == 0) {
         now = next;
         next = scale_at(it + 2 * G);
       }
-      // full implies that the stage's last readers are done
-      if (!mbar_wait(full + 8 * st, (it / ST) & 1)) break;
+      if (!mbar_wait(full + 8 * st, (it / R) & 1)) break;
+      if (it >= G && !mbar_wait(cempty + 8 * g, ((it / G) - 1) & 1)) break;
       uint4 code[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) code[i] = lds16a(base + kQOff + (i * 16 + w * 4 + (lane >> 3)) * kCh + part * 16);
+      for (int i = 0; i < 4; ++i) code[i] = lds16a(src + (i * 16 + w * 4 + (lane >> 3)) * kCh + part * 16);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int t = i * 16 + w * 4 + (lane >> 3);
         const float sc = __shfl_sync(kFull, now, half + i * 4 + (lane >> 3));
-        put_converted<DT>(base, t, part, code[i], sc);
+        put_converted<DT>(dst, t, part, code[i], sc);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(conv + 8 * st);
+      if (lane == 0) {
+        mbar_arrive(conv + 8 * g);
+        mbar_arrive(empty + 8 * st);
+      }
     }
     done = mbar_wait(accf, 0);
     tc_fence_after();
@@ -253,14 +269,17 @@ template <int BN, int DT>
 static cudaError_t launch_wgrad(const void* dy, const void* q, WgradArgs a, int split, cudaStream_t st) {
   CUtensorMap qmap, gmap;
   cudaError_t e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, q, a.K, a.T, a.K, kCh, kTok);
+  constexpr CUtensorMapSwizzle swizzle = BN >= 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                         : BN == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                    : CU_TENSOR_MAP_SWIZZLE_32B;
   if (e == cudaSuccess)
-    e = make_map(&gmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B, dy, a.N, a.T,
-                 static_cast<uint64_t>(a.N) * 2, 64, kTok);
-  if (e == cudaSuccess) e = ensure_smem(int8_wgrad_kernel<BN, DT>, wg_smem(BN));
+    e = make_map(&gmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, swizzle, dy, a.N, a.T, static_cast<uint64_t>(a.N) * 2, wg_width(BN),
+                 kTok);
+  if (e == cudaSuccess) e = ensure_smem(int8_wgrad_kernel<BN, DT>, wg_smem(BN), true);
   if (e != cudaSuccess) return e;
   a.ktiles = (a.K + kCh - 1) / kCh;
   const int tiles = a.ktiles * ((a.N + BN - 1) / BN);
-  return launch_cluster(int8_wgrad_kernel<BN, DT>, dim3(tiles * split), dim3(wg_threads(BN)), wg_smem(BN), split, st, qmap,
+  return launch_cluster(int8_wgrad_kernel<BN, DT>, dim3(tiles * split), dim3(kWgThreads), wg_smem(BN), split, st, qmap,
                         gmap, a, split);
 }
 

@@ -68,13 +68,15 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Shared-memory matrix descriptor, 128-byte swizzle; lbo and sbo in bytes.
-// K-major (rows of 128 bytes along k): sbo = 1024 between groups of 8 rows,
-// lbo unused.  MN-major (rows of 64 16-bit elements along m or n): lbo between
-// groups of 64 elements, sbo = 1024 between groups of 8 k.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+// Shared-memory matrix descriptor; lbo and sbo in bytes.  The rows of 128, 64 or
+// 32 bytes (`row`) are swizzled over as many bytes, in groups of 8.
+// K-major (rows along k): sbo = 8 rows, between groups of 8 of m or n; lbo
+// unused.  MN-major (rows along m or n): lbo between rows' lengths of m or n,
+// sbo = 8 rows, between groups of 8 of k.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, int row = 128) {
+  const uint64_t mode = row == 128 ? 2 : row == 64 ? 4 : 6;
   return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) |
-         (static_cast<uint64_t>(sbo >> 4) << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+         (static_cast<uint64_t>(sbo >> 4) << 32) | (uint64_t{1} << 46) | (mode << 61);
 }
 
 // D[tmem] (+)= A * B, 8-bit integers, 32 k.

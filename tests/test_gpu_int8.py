@@ -327,7 +327,7 @@ def test_empty_tensors(cuda_dev):
 # ---------------------------------------------------------------------- wgrad --
 WGRAD = [(1, 8, 16), (2, 16, 48), (7, 4, 144), (63, 16, 128), (64, 8, 256), (65, 32, 272), (100, 3, 2048), (257, 64, 1040),
          (300, 72, 112), (1000, 16, 2048), (1000, 128, 528), (513, 130, 256), (777, 257, 400), (2048, 512, 512),
-         (4096, 16, 8192), (4097, 264, 1040), (1030, 1000, 2048)]
+         (4096, 16, 8192), (4097, 264, 1040), (1030, 1000, 2048), (200, 2800, 2064), (1000, 1040, 8208), (65, 10000, 528), (130, 24, 8192)]
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
