@@ -35,11 +35,19 @@ __device__ __forceinline__ float load1(const uint16_t* p) {
   return f2lo(unpack2<DT>(w));
 }
 
-// Integer maximum of the bit patterns of non-negative floats: it orders
+// max(m, |lo|, |hi|) in one three-input maximum; NaN stays NaN.
+__device__ __forceinline__ float max_abs_nan(float m, f2_t v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(f2lo(v))), "f"(fabsf(f2hi(v))));
+  return r;
+}
+// Maximum over the warp of bit patterns of non-negative floats: it orders
 // finite < infinity < NaN, so a row with a non-finite value keeps it.
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t max_bits2(uint32_t m, f2_t v) {
-  return max(m, max(abs_bits(f2lo(v)), abs_bits(f2hi(v))));
+// The group's maximum from its warps' in red[0 .. GROUP).
+template <int GROUP>
+__device__ __forceinline__ uint32_t group_max_u32(const uint32_t* red) {
+  const uint32_t v = red[(threadIdx.x & 31) % GROUP];
+  return __reduce_max_sync(kFull, v);
 }
 __device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(kFull, v); }
 
@@ -48,67 +56,57 @@ __device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) { return __reduce_m
 // A row with a non-finite value gets the non-finite scale and zero codes, so
 // whatever is computed from it is NaN.
 //
-// The codes are those of the IEEE quotient RN(RN(127 y) / a) without a
-// division per element: t = y * RN(127 / a) is within 127 * 3 * 2^-24 < 2.3e-5
-// of it, so rint(t) is the code unless t lies within 5e-5 of a half; a vector
-// with such an element takes the division.  For a 16-bit y both 127 y and the
-// ties are exact in fp32, so the code is the exactly rounded one.
+// The quotient is formed without a division, by Markstein's correction ("IA-64
+// and Elementary Functions", 2000): with c = RN(127 y), t1 = RN(y (127 rcp(a)))
+// and the exact remainder r = c - t1 a, t = RN(t1 + r rcp(a)) is c / a to half a
+// unit in its last place and 2^-40.  A 16-bit y makes c exact, a tie c / a =
+// n + 1/2 comes out as itself, and any other quotient is further from a tie
+// than t from the quotient, so the code is the exactly rounded one.  A test of
+// each vector for elements near a tie, with a division for those, took 1.6
+// times as long in all: among 16-bit values exact ties are common.
 struct RowScale {
   float a;    // max(max|y|, 1e-30)
-  float inv;  // 127 / a, or 0 for a row with a non-finite value
-  float s;
+  float rcp;  // 1 / a nearly, or 0 for a row with a non-finite value
+  bool big;   // near the top of the fp32 range: y and a are to be scaled down
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
   RowScale r;
   const float amax = __uint_as_float(amax_bits);
-  if (amax_bits >= 0x7f800000u) {
-    r.a = 1.0f;
-    r.inv = 0.0f;
-    r.s = __fdiv_rn(amax, 127.0f);
-  } else {
-    r.a = fmaxf(amax, 1e-30f);
-    r.inv = __fdiv_rn(127.0f, r.a);
-    r.s = __fdiv_rn(r.a, 127.0f);
-  }
+  const bool finite = amax_bits < 0x7f800000u;
+  r.big = finite && amax > 0x1p100f;
+  r.a = finite ? fmaxf(r.big ? amax * 0x1p-20f : amax, 1e-30f) : 1.0f;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r.rcp) : "f"(r.a));
+  if (!finite) r.rcp = 0.0f;
   return r;
 }
-
-// The quotient for one element.  Rows of values near the top of the fp32
-// range are scaled down by a power of two, which changes no quotient of
-// interest and keeps 127 y finite.
-static __device__ __noinline__ int code_exact(float y, RowScale r) {
-  if (r.inv == 0.0f) return 0;
-  const float k = r.a > 0x1p100f ? 0x1p-20f : 1.0f;
-  return static_cast<int>(rintf(__fdiv_rn(__fmul_rn(127.0f, __fmul_rn(y, k)), __fmul_rn(r.a, k))));
+// The row's scale, from the same maximum.
+__device__ __forceinline__ float scale_value(uint32_t amax_bits) {
+  const float amax = __uint_as_float(amax_bits);
+  return __fdiv_rn(amax_bits < 0x7f800000u ? fmaxf(amax, 1e-30f) : amax, 127.0f);
 }
 
 // Eight codes of four pairs, element k in byte k.
 __device__ __forceinline__ uint2 codes8(const f2_t (&y)[4], const RowScale& r) {
-  const f2_t inv = splat2(r.inv);
+  if (r.rcp == 0.0f) return make_uint2(0, 0);
+  f2_t v[4] = {y[0], y[1], y[2], y[3]};
+  if (r.big) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], splat2(0x1p-20f));
+  }
+  const f2_t inv = splat2(127.0f * r.rcp), rcp = splat2(r.rcp), na = splat2(-r.a);
   const f2_t magic = splat2(12582912.0f);  // 1.5 * 2^23: the sum's low byte is the code
   uint32_t w[8];
-  float far = 0.0f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const f2_t t = mul2(y[j], inv);
-    const f2_t m = add2(t, magic);
-    const f2_t e = sub2(t, sub2(m, magic));
-    far = max_abs2(far, f2lo(e), f2hi(e));
+    const f2_t t1 = mul2(v[j], inv);
+    const f2_t rem = fma2(t1, na, mul2(v[j], splat2(127.0f)));
+    const f2_t m = add2(fma2(rem, rcp, t1), magic);
     w[2 * j] = __float_as_uint(f2lo(m));
     w[2 * j + 1] = __float_as_uint(f2hi(m));
-  }
-  if (far > 0.49995f) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[2 * j] = static_cast<uint32_t>(code_exact(f2lo(y[j]), r));
-      w[2 * j + 1] = static_cast<uint32_t>(code_exact(f2hi(y[j]), r));
-    }
   }
   uint2 o;
   o.x = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
   o.y = __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410);
-  // t is NaN where a non-finite element met the zero factor
-  if (r.inv == 0.0f) o = make_uint2(0, 0);
   return o;
 }
 

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__((GROUP > 4 ? GROUP : 4) * 32) sandwich_fwd_ker
   }
   const float r2 = rms_scale(group_sum(sum, 1), inv_d, a.eps);
   f2_t h[VPL][4];
-  uint32_t top = 0;
+  float amax = 0.0f;
 #pragma unroll
   for (int c = 0; c < VPL; ++c) {
     const int e = (t + 32 * GROUP * c) * 8;
@@ -166,22 +166,21 @@ __global__ void __launch_bounds__((GROUP > 4 ? GROUP : 4) * 32) sandwich_fwd_ker
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           h[c][j] = f2(z[2 * j], z[2 * j + 1]);
-          top = max_bits2(top, h[c][j]);
+          amax = max_abs_nan(amax, h[c][j]);
         }
       }
     }
   }
   if (INT8) {
-    top = warp_max_u32(top);
+    uint32_t top = warp_max_u32(__float_as_uint(amax));
     if (GROUP > 1) {
       if (lane == 0) redu[warp] = top;
       __syncthreads();
-#pragma unroll
-      for (int w = 0; w < GROUP; ++w) top = max(top, redu[w0 + w]);
+      top = group_max_u32<GROUP>(&redu[w0]);
     }
     if (!row_ok) return;
     const RowScale r = row_scale(top);
-    if (t == 0) a.s[row] = r.s;
+    if (t == 0) a.s[row] = scale_value(top);
 #pragma unroll
     for (int c = 0; c < VPL; ++c) {
       const int e = (t + 32 * GROUP * c) * 8;
