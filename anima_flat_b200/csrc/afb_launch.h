@@ -48,6 +48,7 @@ cudaError_t read_status_rms(int* status, bool clear);
 cudaError_t read_status_probe(int* status, bool clear);
 cudaError_t read_status_int8_linear(int* status, bool clear);
 cudaError_t read_status_int8_wgrad(int* status, bool clear);
+cudaError_t read_status_sandwich(int* status, bool clear);
 
 // Column sums of chunk partials part[batch][n][ncols] (fp32) by a stride tree
 // over the chunk index (finalize.cu); column c goes to out[c / seg][b*seg +

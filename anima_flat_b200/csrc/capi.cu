@@ -86,7 +86,8 @@ static int device_status(int* status, bool clear, const char* name) {
   static const Reader readers[] = {afb::read_status_adaln_fwd, afb::read_status_headnorm_fwd,
                                    afb::read_status_headnorm_bwd, afb::read_status_adaln_bwd,
                                    afb::read_status_rms, afb::read_status_probe,
-                                   afb::read_status_int8_linear, afb::read_status_int8_wgrad};
+                                   afb::read_status_int8_linear, afb::read_status_int8_wgrad,
+                                   afb::read_status_sandwich};
   int all = 0;
   for (Reader r : readers) {
     int v = 0;

@@ -85,7 +85,10 @@ __device__ __forceinline__ float scale_value(uint32_t amax_bits) {
   return __fdiv_rn(amax_bits < 0x7f800000u ? fmaxf(amax, 1e-30f) : amax, 127.0f);
 }
 
-// Eight codes of four pairs, element k in byte k.
+// Eight codes of four pairs, element k in byte k.  EXACT: by the corrected
+// quotient; else rint(y (127 rcp(a))), within 3.1e-5 of the quotient, for values
+// that are approximations themselves.
+template <bool EXACT = true>
 __device__ __forceinline__ uint2 codes8(const f2_t (&y)[4], const RowScale& r) {
   if (r.rcp == 0.0f) return make_uint2(0, 0);
   f2_t v[4] = {y[0], y[1], y[2], y[3]};
@@ -99,8 +102,9 @@ __device__ __forceinline__ uint2 codes8(const f2_t (&y)[4], const RowScale& r) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const f2_t t1 = mul2(v[j], inv);
-    const f2_t rem = fma2(t1, na, mul2(v[j], splat2(127.0f)));
-    const f2_t m = add2(fma2(rem, rcp, t1), magic);
+    f2_t t = t1;
+    if (EXACT) t = fma2(fma2(t1, na, mul2(v[j], splat2(127.0f))), rcp, t1);
+    const f2_t m = add2(t, magic);
     w[2 * j] = __float_as_uint(f2lo(m));
     w[2 * j + 1] = __float_as_uint(f2hi(m));
   }

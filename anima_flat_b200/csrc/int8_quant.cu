@@ -96,7 +96,7 @@ rowquant_int8_kernel(const QuantArgs a) {
   for (int c = 0; c < CPL; ++c) {
     const int e = (t + 32 * GROUP * c) * 16;
     if (e >= K) continue;
-    const uint2 lo = codes8(y[c][0], r), hi = codes8(y[c][1], r);
+    const uint2 lo = codes8<MODE != kGelu>(y[c][0], r), hi = codes8<MODE != kGelu>(y[c][1], r);
     st16(a.q + base + e, make_uint4(lo.x, lo.y, hi.x, hi.y));
   }
   if (MODE == kGelu) {

@@ -71,6 +71,16 @@ template <int DT>
 __device__ __forceinline__ uint4 pack8t(const float (&f)[8]) {
   return make_uint4(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]), pack2<DT>(f[6], f[7]));
 }
+template <int DT>
+__device__ __forceinline__ void unpack4p(const uint4 v, f2_t (&f)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = unpack2<DT>(word(v, j));
+}
+template <int DT>
+__device__ __forceinline__ uint4 pack4p(const f2_t (&f)[4]) {
+  return make_uint4(pack2<DT>(f[0]), pack2<DT>(f[1]), pack2<DT>(f[2]), pack2<DT>(f[3]));
+}
+__device__ __forceinline__ float sum2(f2_t v) { return f2lo(v) + f2hi(v); }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
@@ -222,127 +232,247 @@ struct SandwichBwdArgs {
   float alpha, eps;
 };
 
-constexpr int kBwdRows = 2;  // rows a block holds at once
+// A block owns `chunk` rows of one sample.  Its teams of D / 8 threads (rounded
+// up to warps) take pairs of rows in turn; a thread owns 8 columns, whose three
+// sums stay in its registers, so a row is read once.  Bulk copies keep the next
+// two pairs of every team on their way in shared memory: with the loads in the
+// row loop itself the kernel ran at 39% of memory speed, on their latency.
+constexpr int kBwdRows = 2;    // rows a team holds at once
+constexpr int kBwdStages = 3;  // of kBwdRows rows each
+constexpr int kBwdThreads = 512;
+static int bwd_team(int D) { return (D / 8 + 31) / 32 * 32; }
+static int bwd_teams(int D) {
+  const int t = kBwdThreads / bwd_team(D);
+  return t < 8 ? t : 8;
+}
+static size_t bwd_smem(int D) { return static_cast<size_t>(bwd_teams(D)) * kBwdStages * kBwdRows * 4 * D * 2; }
 
-// A block owns `chunk` rows of one sample; a thread owns 8 columns, whose
-// three sums stay in its registers.
+// Sums of eight values over the warp: lane l returns that of value l / 4.
+// Each step halves the values a lane carries, 9 exchanges for the 40 of eight
+// butterflies.
+__device__ __forceinline__ float warp_sum8(const float (&v)[8]) {
+  const int lane = threadIdx.x & 31;
+  float a[4], b[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool up = lane & 16;
+    a[i] = (up ? v[i + 4] : v[i]) + __shfl_xor_sync(kFull, up ? v[i] : v[i + 4], 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool up = lane & 8;
+    b[i] = (up ? a[i + 2] : a[i]) + __shfl_xor_sync(kFull, up ? a[i] : a[i + 2], 8);
+  }
+  const bool up = lane & 4;
+  float c = (up ? b[1] : b[0]) + __shfl_xor_sync(kFull, up ? b[0] : b[1], 4);
+  c += __shfl_xor_sync(kFull, c, 2);
+  return c + __shfl_xor_sync(kFull, c, 1);
+}
+// Sums of two values: lane l returns that of value l / 16.
+__device__ __forceinline__ float warp_sum2(float v0, float v1) {
+  const bool up = threadIdx.x & 16;
+  float c = (up ? v1 : v0) + __shfl_xor_sync(kFull, up ? v0 : v1, 16);
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) c += __shfl_xor_sync(kFull, c, o);
+  return c;
+}
+// The team's sum of value l / 4 or l / 16, for every lane l, from its warps' in
+// red[value][warp] (zero above the team's warps).
+__device__ __forceinline__ float team_sum8(const float (*red)[16]) {
+  const int lane = threadIdx.x & 31;
+  const float4 p = *reinterpret_cast<const float4*>(&red[lane >> 2][4 * (lane & 3)]);
+  float c = (p.x + p.y) + (p.z + p.w);
+  c += __shfl_xor_sync(kFull, c, 2);
+  return c + __shfl_xor_sync(kFull, c, 1);
+}
+__device__ __forceinline__ float team_sum2(const float (*red)[16]) {
+  const int lane = threadIdx.x & 31;
+  float c = red[lane >> 4][lane & 15];
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) c += __shfl_xor_sync(kFull, c, o);
+  return c;
+}
+
 template <int DT>
-__global__ void __launch_bounds__(512) sandwich_bwd_kernel(const SandwichBwdArgs a) {
-  constexpr int R = kBwdRows;
-  __shared__ float red[2][R][4][16];
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  const int e = threadIdx.x * 8;
+__global__ void __launch_bounds__(kBwdThreads, 1) sandwich_bwd_kernel(const SandwichBwdArgs a, int team_threads, int teams) {
+  constexpr int R = kBwdRows, NS = kBwdStages;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ __align__(8) uint64_t bars[8 * NS];
+  // per team: sums of z^2, p z, x^2 of the rows by warp, and of m xh
+  __shared__ __align__(16) float red1[8][8][16], red2[8][R][16];
+  const int lane = threadIdx.x & 31;
+  const int team = static_cast<int>(threadIdx.x) / team_threads, tid = static_cast<int>(threadIdx.x) % team_threads;
+  const int warp = tid >> 5;
+  const int e = tid * 8;
   const bool col = e < a.D;
   const int64_t b = blockIdx.y, r0 = static_cast<int64_t>(blockIdx.x) * a.chunk;
-  const int64_t r1 = min(r0 + a.chunk, a.S);
+  const int rows = static_cast<int>(min(static_cast<int64_t>(a.chunk), a.S - r0));
   const float inv_d = __fdiv_rn(1.0f, static_cast<float>(a.D));
-  float gw[8] = {}, pw[8] = {};  // gate * post, scale * pre
+  const uint32_t row_bytes = static_cast<uint32_t>(a.D) * 2, stage_bytes = R * 4 * row_bytes;
+  const uint32_t ring = smem_addr(dyn) + team * NS * stage_bytes, bar0 = smem_addr(bars) + team * NS * 8;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(bar0 + 8 * i, 1);
+    fence_mbar_init();
+  }
+  for (int i = static_cast<int>(threadIdx.x); i < 8 * 8 * 16; i += static_cast<int>(blockDim.x)) {
+    (&red1[0][0][0])[i] = 0.0f;
+    if (i < 8 * R * 16) (&red2[0][0][0])[i] = 0.0f;
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+
+  // Pair i of the team: rows (i * teams + team) * R of the chunk.
+  const int pairs = (rows + R - 1) / R;
+  const int mine = pairs > team ? (pairs - team + teams - 1) / teams : 0;
+  const uint16_t* src[4] = {a.gh, a.gz, a.z, a.x};
+  auto request = [&](int i) {
+    const int r = (i * teams + team) * R, n = min(R, rows - r);
+    const uint32_t bar = bar0 + 8 * (i % NS), dst = ring + (i % NS) * stage_bytes;
+    mbar_arrive_expect_tx(bar, n * (a.gz ? 4 : 3) * row_bytes);
+    for (int k = 0; k < n; ++k)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (src[t] != nullptr)
+          bulk_g2s(dst + (k * 4 + t) * row_bytes, src[t] + (b * a.S + r0 + r + k) * a.D, row_bytes, bar);
+  };
+  int asked = 0;
+  if (tid == 0)
+    for (; asked < NS - 1 && asked < mine; ++asked) request(asked);
+
+  f2_t gw[4] = {}, pw[4] = {};  // gate * post, scale * pre
   if (col) {
-    float u[8];
-    load8<DT>(a.gate ? a.gate + b * a.D + e : nullptr, 1.0f, gw);
+    float u[8], v[8];
+    load8<DT>(a.gate ? a.gate + b * a.D + e : nullptr, 1.0f, v);
     load8f(a.post + e, u);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) gw[k] *= u[k];
-    load8<DT>(a.scale ? a.scale + b * a.D + e : nullptr, 1.0f, pw);
+    for (int j = 0; j < 4; ++j) gw[j] = mul2(f2(u[2 * j], u[2 * j + 1]), f2(v[2 * j], v[2 * j + 1]));
+    load8<DT>(a.scale ? a.scale + b * a.D + e : nullptr, 1.0f, v);
     load8f(a.pre + e, u);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) pw[k] *= u[k];
+    for (int j = 0; j < 4; ++j) pw[j] = mul2(f2(u[2 * j], u[2 * j + 1]), f2(v[2 * j], v[2 * j + 1]));
   }
-  float P[8] = {}, Q[8] = {}, G[8] = {};
-  for (int64_t r = r0; r < r1; r += R) {
-    uint4 ghv[R], gzv[R], zv[R], xv[R];
+  f2_t P[4] = {}, Q[4] = {}, G[4] = {};
+  bool ok = true;
+  const f2_t alpha = splat2(a.alpha);
+  for (int i = 0; i < mine; ++i) {
+    const int r = (i * teams + team) * R;
+    // A thread reads its own 16 bytes of each row alone; one past the last
+    // column reads column 0 and counts nothing.
+    uint8_t* at = dyn + (team * NS + i % NS) * stage_bytes + (col ? tid * 16 : 0);
+    auto piece = [&](int k, int t) -> uint8_t* { return at + (k * 4 + t) * row_bytes; };
+    ok = ok && mbar_wait(bar0 + 8 * (i % NS), (i / NS) & 1);
+    if (col) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const bool ok = col && r + i < r1;
-      const int64_t at = (b * a.S + r + i) * a.D + e;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      ghv[i] = ok ? ld_stream(a.gh + at) : zero;
-      gzv[i] = ok && a.gz ? ld_stream(a.gz + at) : zero;
-      zv[i] = ok ? ld_stream(a.z + at) : zero;
-      xv[i] = ok ? ld_stream(a.x + at) : zero;
-    }
+      for (int k = 0; k < R; ++k) {
+        if (r + k < rows) continue;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float g[8], z[8], x[8], s0 = 0.0f, s1 = 0.0f, s2 = 0.0f;
-      unpack8t<DT>(ghv[i], g);
-      unpack8t<DT>(zv[i], z);
-      unpack8t<DT>(xv[i], x);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        s0 = __fmaf_rn(z[k], z[k], s0);
-        s1 = __fmaf_rn(g[k] * pw[k], z[k], s1);
-        s2 = __fmaf_rn(x[k], x[k], s2);
-      }
-      s0 = warp_sum(s0);
-      s1 = warp_sum(s1);
-      s2 = warp_sum(s2);
-      if (lane == 0) {
-        red[0][i][0][warp] = s0;
-        red[0][i][1][warp] = s1;
-        red[0][i][2][warp] = s2;
+        for (int t = 0; t < 4; ++t) st16(piece(k, t), make_uint4(0, 0, 0, 0));  // no such row
       }
     }
-    __syncthreads();
-    float dz[R][8], rx[R];
+    float sums[8] = {};
+    if (col) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
-      for (int w = 0; w < nw; ++w) {
-        s0 += red[0][i][0][w];
-        s1 += red[0][i][1][w];
-        s2 += red[0][i][2][w];
-      }
-      const float rz = rms_scale(s0, inv_d, a.eps);
-      rx[i] = rms_scale(s2, inv_d, a.eps);
-      const float c = s1 * rz * inv_d;  // mean(p zh)
-      float g[8], z[8], x[8], gz[8];
-      unpack8t<DT>(ghv[i], g);
-      unpack8t<DT>(zv[i], z);
-      unpack8t<DT>(xv[i], x);
-      unpack8t<DT>(gzv[i], gz);
+      for (int k = 0; k < R; ++k) {
+        f2_t g[4], z[4], x[4], s0 = 0, s1 = 0, s2 = 0;
+        unpack4p<DT>(lds16(piece(k, 0)), g);
+        unpack4p<DT>(lds16(piece(k, 2)), z);
+        unpack4p<DT>(lds16(piece(k, 3)), x);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float zh = z[k] * rz, xh = x[k] * rx[i];
-        dz[i][k] = __fmaf_rn(rz, __fmaf_rn(-zh, c, g[k] * pw[k]), gz[k]);
-        s3 = __fmaf_rn(dz[i][k] * gw[k], xh, s3);
-        P[k] = __fmaf_rn(g[k], zh, P[k]);
-        Q[k] = __fmaf_rn(dz[i][k], xh, Q[k]);
-        G[k] += g[k];
-      }
-      s3 = warp_sum(s3);
-      if (lane == 0) red[1][i][3][warp] = s3;
-      if (col && r + i < r1) {
-        float o[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = a.alpha * dz[i][k];
-        st16(a.dres + (b * a.S + r + i) * a.D + e, pack8t<DT>(o));
+        for (int j = 0; j < 4; ++j) {
+          s0 = fma2(z[j], z[j], s0);
+          s1 = fma2(mul2(g[j], pw[j]), z[j], s1);
+          s2 = fma2(x[j], x[j], s2);
+        }
+        sums[k] = sum2(s0);
+        sums[2 + k] = sum2(s2);
+        sums[4 + k] = sum2(s1);
       }
     }
-    __syncthreads();
+    const float own = warp_sum8(sums);
+    if ((lane & 3) == 0) red1[team][lane >> 2][warp] = own;
+    named_bar_sync(1 + team, team_threads);
+    // The team is done with pair i - 1: its stage takes pair i + 2.
+    if (tid == 0 && ok && asked < mine) {
+      fence_proxy_async_smem();
+      request(asked++);
+    }
+    // Lanes of the first four values turn them into reciprocal roots; the
+    // last two become the means of p zh.
+    const float all = team_sum8(red1[team]);
+    const float root = rsqrtf(__fmaf_rn(all, inv_d, a.eps));
+    f2_t dm[R][4];  // dz gate post
+    float rx[R], part[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float s3 = 0.0f;
-      for (int w = 0; w < nw; ++w) s3 += red[1][i][3][w];
-      const float c = s3 * inv_d;
-      if (col && r + i < r1) {
-        float x[8];
-        unpack8t<DT>(xv[i], x);
+    for (int k = 0; k < R; ++k) {
+      const float rz = __shfl_sync(kFull, root, 4 * k);
+      rx[k] = __shfl_sync(kFull, root, 8 + 4 * k);
+      const float c = __shfl_sync(kFull, all, 16 + 4 * k) * rz * inv_d;  // mean(p zh)
+      f2_t g[4], z[4], x[4], gz[4] = {}, o[4], s3 = 0;
+      unpack4p<DT>(lds16(piece(k, 0)), g);
+      if (a.gz != nullptr) unpack4p<DT>(lds16(piece(k, 1)), gz);
+      unpack4p<DT>(lds16(piece(k, 2)), z);
+      unpack4p<DT>(lds16(piece(k, 3)), x);
+      const f2_t rz2 = splat2(rz), rx2 = splat2(rx[k]), nc = splat2(-c);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = rx[i] * __fmaf_rn(-(x[k] * rx[i]), c, dz[i][k] * gw[k]);
-        st16(a.dx + (b * a.S + r + i) * a.D + e, pack8t<DT>(x));
+      for (int j = 0; j < 4; ++j) {
+        const f2_t zh = mul2(z[j], rz2), xh = mul2(x[j], rx2);
+        const f2_t dz = fma2(rz2, fma2(zh, nc, mul2(g[j], pw[j])), gz[j]);
+        dm[k][j] = mul2(dz, gw[j]);
+        s3 = fma2(dm[k][j], xh, s3);
+        P[j] = fma2(g[j], zh, P[j]);
+        Q[j] = fma2(dz, xh, Q[j]);
+        G[j] = add2(G[j], g[j]);
+        o[j] = mul2(alpha, dz);
+      }
+      part[k] = col ? sum2(s3) : 0.0f;
+      if (col && r + k < rows) st16(a.dres + (b * a.S + r0 + r + k) * a.D + e, pack4p<DT>(o));
+    }
+    const float own2 = warp_sum2(part[0], part[1]);
+    if ((lane & 15) == 0) red2[team][lane >> 4][warp] = own2;
+    named_bar_sync(1 + team, team_threads);
+    const float mean = team_sum2(red2[team]) * inv_d;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const f2_t nc = splat2(-__shfl_sync(kFull, mean, 16 * k)), rx2 = splat2(rx[k]);
+      if (col && r + k < rows) {
+        f2_t x[4];
+        unpack4p<DT>(lds16(piece(k, 3)), x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = mul2(rx2, fma2(mul2(x[j], rx2), nc, dm[k][j]));
+        st16(a.dx + (b * a.S + r0 + r + k) * a.D + e, pack4p<DT>(x));
       }
     }
   }
-  if (col) {
-    float* p = a.part + (b * gridDim.x + blockIdx.x) * 3 * a.D + e;
+  // After a wait that gave up: copies in flight land before the block ends.
+  if (tid == 0 && !ok)
+    for (int i = asked > NS ? asked - NS : 0; i < asked; ++i) mbar_wait(bar0 + 8 * (i % NS), (i / NS) & 1);
+
+  // The teams' column sums, in order, through the ring.
+  f2_t* sums[3] = {P, Q, G};
+  if (teams > 1) {
+    f2_t* f = reinterpret_cast<f2_t*>(dyn);
+    const int half = a.D / 2;
+    __syncthreads();
+    if (team > 0 && col)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      p[k] = P[k];
-      p[a.D + k] = Q[k];
-      p[2 * a.D + k] = G[k];
-    }
+      for (int n = 0; n < 3; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[((team - 1) * 3 + n) * half + tid * 4 + j] = sums[n][j];
+    __syncthreads();
+    if (team == 0 && col)
+      for (int t = 0; t + 1 < teams; ++t)
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sums[n][j] = add2(sums[n][j], f[(t * 3 + n) * half + tid * 4 + j]);
+  }
+  if (team == 0 && col) {
+    f2_t* p = reinterpret_cast<f2_t*>(a.part + (b * gridDim.x + blockIdx.x) * 3 * a.D + e);
+#pragma unroll
+    for (int n = 0; n < 3; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[n * (a.D / 2) + j] = sums[n][j];
   }
 }
 
@@ -356,56 +486,58 @@ struct SandwichFinalArgs {
   int chunks, D;
 };
 
-// 32 columns a block; its 32 warps each sum every 32nd chunk.
+// 32 columns a block; its 32 warps each sum every 32nd chunk, lane by column,
+// then each adds the warps' sums of one column.
 template <int DT>
 __global__ void __launch_bounds__(1024) sandwich_final_kernel(const SandwichFinalArgs a) {
-  __shared__ float red[32][3][33];
+  __shared__ float red[3][32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cl = blockIdx.x * 32 + lane, cw = blockIdx.x * 32 + warp;
+  const bool last = lane == 0 && cw < a.D;
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
-  const bool ok = c < a.D;
+  const float post = last ? __ldg(a.post + cw) : 0.0f, pre = last ? __ldg(a.pre + cw) : 0.0f;
   float dpost = 0.0f, dpre = 0.0f;
   for (int64_t b = 0; b < a.B; ++b) {
+    const int64_t at = b * a.D + cw;
+    const float scale = last && a.scale ? load1<DT>(a.scale + at) : 1.0f;
+    const float gate = last && a.gate ? load1<DT>(a.gate + at) : 1.0f;
     float s[3] = {};
-    if (ok) {
+    if (cl < a.D) {
+#pragma unroll 4
       for (int n = warp; n < a.chunks; n += 32) {
-        const float* p = a.part + (b * a.chunks + n) * 3 * a.D + c;
+        const float* p = a.part + (b * a.chunks + n) * 3 * a.D + cl;
 #pragma unroll
         for (int i = 0; i < 3; ++i) s[i] += __ldg(p + static_cast<int64_t>(i) * a.D);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) red[warp][i][lane] = s[i];
+    for (int i = 0; i < 3; ++i) red[i][warp][lane] = s[i];
     __syncthreads();
-    if (warp == 0 && ok) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        s[i] = 0.0f;
-        for (int w = 0; w < 32; ++w) s[i] += red[w][i][lane];
-      }
-      const int64_t at = b * a.D + c;
-      dpre = __fmaf_rn(a.scale ? load1<DT>(a.scale + at) : 1.0f, s[0], dpre);
-      dpost = __fmaf_rn(a.gate ? load1<DT>(a.gate + at) : 1.0f, s[1], dpost);
-      if (a.dscale) a.dscale[at] = static_cast<uint16_t>(pack2<DT>(a.pre[c] * s[0], 0.0f));
-      if (a.dgate) a.dgate[at] = static_cast<uint16_t>(pack2<DT>(a.post[c] * s[1], 0.0f));
+    for (int i = 0; i < 3; ++i) s[i] = warp_sum(red[i][lane][warp]);
+    __syncthreads();
+    if (last) {
+      dpre = __fmaf_rn(scale, s[0], dpre);
+      dpost = __fmaf_rn(gate, s[1], dpost);
+      if (a.dscale) a.dscale[at] = static_cast<uint16_t>(pack2<DT>(pre * s[0], 0.0f));
+      if (a.dgate) a.dgate[at] = static_cast<uint16_t>(pack2<DT>(post * s[1], 0.0f));
       if (a.dshift) a.dshift[at] = static_cast<uint16_t>(pack2<DT>(s[2], 0.0f));
     }
-    __syncthreads();
   }
-  if (warp == 0 && ok) {
-    a.dpost[c] = dpost;
-    a.dpre[c] = dpre;
+  if (last) {
+    a.dpost[cw] = dpost;
+    a.dpre[cw] = dpre;
   }
 }
 
-// Rows of a backward block: enough blocks for two a multiprocessor, and no
-// fewer than 8 rows each, so that the column sums that a block leaves stay
-// below its rows' own traffic.  148 multiprocessors, whatever the device.
-static int64_t bwd_chunk(int64_t B, int64_t S) {
-  const int64_t per = (B * S + 295) / 296;
-  const int64_t c = ((per < 8 ? 8 : per) + kBwdRows - 1) / kBwdRows * kBwdRows;
-  return c < S ? c : S;
+// Rows of a backward block: one block a multiprocessor (148, whatever the
+// device: the sums' order follows from the sizes alone), of at least one pair
+// of rows for each team.
+static int64_t bwd_chunk(int64_t B, int64_t S, int64_t D) {
+  const int64_t per_sample = B < 148 ? 148 / B : 1;
+  const int64_t c = (S + per_sample - 1) / per_sample, least = bwd_teams(static_cast<int>(D)) * kBwdRows;
+  return c > least ? c : least;
 }
 static bool check_sandwich(int64_t B, int64_t S, int64_t D, int dtype) {
   return check(B >= 0 && B <= 65535, "batch must be in [0, 65535]") &&
@@ -418,6 +550,8 @@ static bool check_sandwich(int64_t B, int64_t S, int64_t D, int dtype) {
 static bool check_opt16(const void* p, const char* n) {
   return check(aligned(p, 16), std::string(n) + " is not 16-byte aligned");
 }
+
+cudaError_t read_status_sandwich(int* status, bool clear) { return tu_status(status, clear); }
 
 }  // namespace afb
 
@@ -475,8 +609,8 @@ extern "C" int afb_sandwich_norm_int8(const void* x, const void* residual, const
 
 extern "C" size_t afb_sandwich_norm_bwd_workspace(int64_t batch, int64_t seq, int64_t dim) {
   if (batch <= 0 || seq <= 0 || dim <= 0) return 0;
-  if (batch > 65535 || seq > (1 << 30) || dim > kMaxRowDim) return SIZE_MAX;
-  const int64_t c = bwd_chunk(batch, seq);
+  if (batch > 65535 || seq > (1 << 30) || dim > kMaxRowDim || dim % 8 != 0) return SIZE_MAX;
+  const int64_t c = bwd_chunk(batch, seq, dim);
   return static_cast<size_t>(batch * ((seq + c - 1) / c) * 3 * dim) * sizeof(float);
 }
 
@@ -505,7 +639,7 @@ extern "C" int afb_sandwich_norm_bwd(const void* gh, const void* gz, const void*
   a.dres = static_cast<uint16_t*>(dres);
   a.part = static_cast<float*>(workspace);
   a.S = seq;
-  a.chunk = static_cast<int>(bwd_chunk(batch, seq));
+  a.chunk = static_cast<int>(bwd_chunk(batch, seq, dim));
   a.D = static_cast<int>(dim);
   a.alpha = residual_scale;
   a.eps = eps;
@@ -525,9 +659,13 @@ extern "C" int afb_sandwich_norm_bwd(const void* gh, const void* gz, const void*
   f.D = a.D;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(f.chunks), static_cast<unsigned>(batch));
-  const dim3 block(static_cast<unsigned>((dim / 8 + 31) / 32 * 32));
-  cudaError_t e = dtype == kBf16 ? launch_pdl(sandwich_bwd_kernel<kBf16>, grid, block, 0, st, a)
-                                 : launch_pdl(sandwich_bwd_kernel<kFp16>, grid, block, 0, st, a);
+  const int team = bwd_team(a.D), teams = bwd_teams(a.D);
+  const dim3 block(static_cast<unsigned>(team * teams));
+  const size_t smem = bwd_smem(a.D);
+  cudaError_t e = dtype == kBf16 ? ensure_smem(sandwich_bwd_kernel<kBf16>, smem) : ensure_smem(sandwich_bwd_kernel<kFp16>, smem);
+  if (e != cudaSuccess) return g.done(e);
+  e = dtype == kBf16 ? launch_pdl(sandwich_bwd_kernel<kBf16>, grid, block, smem, st, a, team, teams)
+                     : launch_pdl(sandwich_bwd_kernel<kFp16>, grid, block, smem, st, a, team, teams);
   if (e != cudaSuccess) return g.done(e);
   const dim3 fg(static_cast<unsigned>((dim + 31) / 32));
   return g.done(dtype == kBf16 ? launch_pdl(sandwich_final_kernel<kBf16>, fg, dim3(1024), 0, st, f)
