@@ -38,6 +38,25 @@ struct SandwichArgs {
   float alpha, eps;
 };
 
+// The same as pairs.
+template <int DT>
+__device__ __forceinline__ void load4p(const uint16_t* p, float fallback, f2_t (&f)[4]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = splat2(fallback);
+    return;
+  }
+  const uint4 v = ld_keep(p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = unpack2<DT>(word(v, j));
+}
+__device__ __forceinline__ void load4pf(const float* p, f2_t (&f)[4]) {
+  const ulonglong2 lo = __ldg(reinterpret_cast<const ulonglong2*>(p)), hi = __ldg(reinterpret_cast<const ulonglong2*>(p + 4));
+  f[0] = lo.x;
+  f[1] = lo.y;
+  f[2] = hi.x;
+  f[3] = hi.y;
+}
 template <int DT>
 __device__ __forceinline__ void load8(const uint16_t* p, float fallback, float (&f)[8]) {
   if (p == nullptr) {
@@ -59,19 +78,6 @@ __device__ __forceinline__ void load8f(const float* p, float (&f)[8]) {
   f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
 }
 template <int DT>
-__device__ __forceinline__ void unpack8t(const uint4 v, float (&f)[8]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const f2_t t = unpack2<DT>(word(v, j));
-    f[2 * j] = f2lo(t);
-    f[2 * j + 1] = f2hi(t);
-  }
-}
-template <int DT>
-__device__ __forceinline__ uint4 pack8t(const float (&f)[8]) {
-  return make_uint4(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]), pack2<DT>(f[6], f[7]));
-}
-template <int DT>
 __device__ __forceinline__ void unpack4p(const uint4 v, f2_t (&f)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) f[j] = unpack2<DT>(word(v, j));
@@ -87,7 +93,7 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 __device__ __forceinline__ float rms_scale(float sum, float inv_d, float eps) {
-  return __fdiv_rn(1.0f, __fsqrt_rn(__fmaf_rn(sum, inv_d, eps)));
+  return rsqrtf(__fmaf_rn(sum, inv_d, eps));
 }
 
 // ------------------------------------------------------------------ forward --
@@ -128,57 +134,52 @@ __global__ void __launch_bounds__((GROUP > 4 ? GROUP : 4) * 32) sandwich_fwd_ker
     xv[c] = ok ? ld_stream(a.x + base + e) : make_uint4(0, 0, 0, 0);
     zv[c] = ok ? ld_stream(a.res + base + e) : make_uint4(0, 0, 0, 0);
   }
-  float sum = 0.0f;
+  f2_t sum = 0;
 #pragma unroll
   for (int c = 0; c < VPL; ++c) {
-    float f[8];
-    unpack8t<DT>(xv[c], f);
+    f2_t f[4];
+    unpack4p<DT>(xv[c], f);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum = __fmaf_rn(f[k], f[k], sum);
+    for (int j = 0; j < 4; ++j) sum = fma2(f[j], f[j], sum);
   }
-  const float r1 = rms_scale(group_sum(sum, 0), inv_d, a.eps);
-  sum = 0.0f;
+  const f2_t r1 = splat2(rms_scale(group_sum(sum2(sum), 0), inv_d, a.eps)), alpha = splat2(a.alpha);
+  sum = 0;
 #pragma unroll
   for (int c = 0; c < VPL; ++c) {
     const int e = (t + 32 * GROUP * c) * 8;
     if (row_ok && e < a.D) {
-      float x[8], r[8], g[8], p[8];
-      unpack8t<DT>(xv[c], x);
-      unpack8t<DT>(zv[c], r);
-      load8<DT>(a.gate ? a.gate + bd + e : nullptr, 1.0f, g);
-      load8f(a.post + e, p);
+      f2_t x[4], r[4], g[4], p[4];
+      unpack4p<DT>(xv[c], x);
+      unpack4p<DT>(zv[c], r);
+      load4p<DT>(a.gate ? a.gate + bd + e : nullptr, 1.0f, g);
+      load4pf(a.post + e, p);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) r[k] = __fmaf_rn(g[k], x[k] * r1 * p[k], a.alpha * r[k]);
-      zv[c] = pack8t<DT>(r);
+      for (int j = 0; j < 4; ++j) r[j] = fma2(mul2(g[j], p[j]), mul2(x[j], r1), mul2(alpha, r[j]));
+      zv[c] = pack4p<DT>(r);
       st16(a.z + base + e, zv[c]);
-      unpack8t<DT>(zv[c], r);
+      unpack4p<DT>(zv[c], r);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum = __fmaf_rn(r[k], r[k], sum);
+      for (int j = 0; j < 4; ++j) sum = fma2(r[j], r[j], sum);
     }
   }
-  const float r2 = rms_scale(group_sum(sum, 1), inv_d, a.eps);
+  const f2_t r2 = splat2(rms_scale(group_sum(sum2(sum), 1), inv_d, a.eps));
   f2_t h[VPL][4];
   float amax = 0.0f;
 #pragma unroll
   for (int c = 0; c < VPL; ++c) {
     const int e = (t + 32 * GROUP * c) * 8;
     if (row_ok && e < a.D) {
-      float z[8], p[8], sc[8], sh[8];
-      unpack8t<DT>(zv[c], z);
-      load8f(a.pre + e, p);
-      load8<DT>(a.scale ? a.scale + bd + e : nullptr, 1.0f, sc);
-      load8<DT>(a.shift ? a.shift + bd + e : nullptr, 0.0f, sh);
+      f2_t z[4], p[4], sc[4], sh[4];
+      unpack4p<DT>(zv[c], z);
+      load4pf(a.pre + e, p);
+      load4p<DT>(a.scale ? a.scale + bd + e : nullptr, 1.0f, sc);
+      load4p<DT>(a.shift ? a.shift + bd + e : nullptr, 0.0f, sh);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) z[k] = __fmaf_rn(z[k] * r2 * p[k], sc[k], sh[k]);
-      if (!INT8) {
-        st16(a.h + base + e, pack8t<DT>(z));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          h[c][j] = f2(z[2 * j], z[2 * j + 1]);
-          amax = max_abs_nan(amax, h[c][j]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        h[c][j] = fma2(mul2(z[j], r2), mul2(p[j], sc[j]), sh[j]);
+        if (INT8) amax = max_abs_nan(amax, h[c][j]);
       }
+      if (!INT8) st16(a.h + base + e, pack4p<DT>(h[c]));
     }
   }
   if (INT8) {
@@ -199,6 +200,214 @@ __global__ void __launch_bounds__((GROUP > 4 ? GROUP : 4) * 32) sandwich_fwd_ker
   }
 }
 
+// Many rows: a block owns a chunk of one sample's rows, its teams of D / 8
+// threads take four rows at a time.  A thread owns 8 columns and keeps their
+// factors in registers; in the kernel above every row reads them again, 14 bytes
+// an element from L1 for 8 from memory.  Bulk copies keep the next rows coming.
+constexpr int64_t kManyRows = 2048;
+constexpr int kFwdRows = 4;
+constexpr int kFwdStages = 3;
+constexpr int kTeamThreads = 512;
+static int team_threads_of(int D) { return (D / 8 + 31) / 32 * 32; }
+static int teams_of(int D) {
+  const int t = kTeamThreads / team_threads_of(D);
+  return t < 8 ? t : 8;
+}
+static size_t fwd_smem(int D) { return static_cast<size_t>(teams_of(D)) * kFwdStages * kFwdRows * 2 * D * 2; }
+
+// Sums, or maxima of bit patterns, of four values over the warp: lane l returns
+// that of value l / 8.
+__device__ __forceinline__ float warp_sum4(const float (&v)[4]) {
+  const int lane = threadIdx.x & 31;
+  float b[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool up = lane & 16;
+    b[i] = (up ? v[i + 2] : v[i]) + __shfl_xor_sync(kFull, up ? v[i] : v[i + 2], 16);
+  }
+  const bool up = lane & 8;
+  float c = (up ? b[1] : b[0]) + __shfl_xor_sync(kFull, up ? b[0] : b[1], 8);
+#pragma unroll
+  for (int o = 4; o >= 1; o >>= 1) c += __shfl_xor_sync(kFull, c, o);
+  return c;
+}
+// The team's sum of value l / 8 from its warps' in red[value][warp].
+__device__ __forceinline__ float team_sum4(const float (*red)[16]) {
+  const int lane = threadIdx.x & 31;
+  const float2 p = *reinterpret_cast<const float2*>(&red[lane >> 3][2 * (lane & 7)]);
+  float c = p.x + p.y;
+#pragma unroll
+  for (int o = 4; o >= 1; o >>= 1) c += __shfl_xor_sync(kFull, c, o);
+  return c;
+}
+
+template <int DT, bool INT8>
+__global__ void __launch_bounds__(kTeamThreads, 1)
+sandwich_rows_kernel(const SandwichArgs a, int64_t S, int chunk, int team_threads, int teams) {
+  constexpr int R = kFwdRows, NS = kFwdStages;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ __align__(8) uint64_t bars[8 * NS];
+  __shared__ __align__(16) float red[2][8][R][16];
+  __shared__ uint32_t redu[8][R][16];
+  const int lane = threadIdx.x & 31;
+  const int team = static_cast<int>(threadIdx.x) / team_threads, tid = static_cast<int>(threadIdx.x) % team_threads;
+  const int warp = tid >> 5, e = tid * 8;
+  const bool col = e < a.D;
+  const int64_t b = blockIdx.y, r0 = static_cast<int64_t>(blockIdx.x) * chunk;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(chunk), S - r0));
+  const float inv_d = __fdiv_rn(1.0f, static_cast<float>(a.D));
+  const uint32_t row_bytes = static_cast<uint32_t>(a.D) * 2, stage_bytes = R * 2 * row_bytes;
+  const uint32_t ring = smem_addr(dyn) + team * NS * stage_bytes, bar0 = smem_addr(bars) + team * NS * 8;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(bar0 + 8 * i, 1);
+    fence_mbar_init();
+  }
+  for (int i = static_cast<int>(threadIdx.x); i < 8 * R * 16; i += static_cast<int>(blockDim.x)) {
+    (&red[0][0][0][0])[i] = (&red[1][0][0][0])[i] = 0.0f;
+    (&redu[0][0][0])[i] = 0;
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+
+  // Group i of the team: rows (i * teams + team) * R of the chunk.
+  const int groups = (rows + R - 1) / R;
+  const int mine = groups > team ? (groups - team + teams - 1) / teams : 0;
+  auto request = [&](int i) {
+    const int r = (i * teams + team) * R, n = min(R, rows - r);
+    const uint32_t bar = bar0 + 8 * (i % NS), dst = ring + (i % NS) * stage_bytes;
+    const int64_t at = (b * S + r0 + r) * a.D;
+    mbar_arrive_expect_tx(bar, n * 2 * row_bytes);
+    bulk_g2s(dst, a.x + at, n * row_bytes, bar);  // neighbouring rows are one piece
+    bulk_g2s(dst + R * row_bytes, a.res + at, n * row_bytes, bar);
+  };
+  int asked = 0;
+  if (tid == 0)
+    for (; asked < NS - 1 && asked < mine; ++asked) request(asked);
+
+  f2_t gp[4] = {}, ps[4] = {}, sh[4] = {};  // gate * post, pre * scale, shift
+  if (col) {
+    f2_t u[4];
+    load4pf(a.post + e, u);
+    load4p<DT>(a.gate ? a.gate + b * a.D + e : nullptr, 1.0f, gp);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) gp[j] = mul2(gp[j], u[j]);
+    load4pf(a.pre + e, u);
+    load4p<DT>(a.scale ? a.scale + b * a.D + e : nullptr, 1.0f, ps);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ps[j] = mul2(ps[j], u[j]);
+    load4p<DT>(a.shift ? a.shift + b * a.D + e : nullptr, 0.0f, sh);
+  }
+  const f2_t alpha = splat2(a.alpha);
+  bool ok = true;
+  for (int i = 0; i < mine; ++i) {
+    const int r = (i * teams + team) * R;
+    // A thread reads its own 16 bytes of each row alone; one past the last
+    // column reads column 0 and counts nothing.
+    const uint8_t* at = dyn + (team * NS + i % NS) * stage_bytes + (col ? tid * 16 : 0);
+    ok = ok && mbar_wait(bar0 + 8 * (i % NS), (i / NS) & 1);
+    const int64_t out = (b * S + r0 + r) * a.D + e;
+    float part[R];
+    uint4 xv[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      // rows past the chunk's last hold what was there: they are not written
+      f2_t x[4], s = 0;
+      xv[k] = lds16(at + k * row_bytes);
+      unpack4p<DT>(xv[k], x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fma2(x[j], x[j], s);
+      part[k] = col ? sum2(s) : 0.0f;
+    }
+    const float own = warp_sum4(part);
+    if ((lane & 7) == 0) red[0][team][lane >> 3][warp] = own;
+    named_bar_sync(1 + team, team_threads);
+    // The team is done with group i - 1: its stage takes group i + 2.
+    if (tid == 0 && ok && asked < mine) {
+      fence_proxy_async_smem();
+      request(asked++);
+    }
+    const float root = rms_scale(team_sum4(red[0][team]), inv_d, a.eps);
+    uint4 zv[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const f2_t r1 = splat2(__shfl_sync(kFull, root, 8 * k));
+      f2_t x[4], z[4], s = 0;
+      unpack4p<DT>(xv[k], x);
+      unpack4p<DT>(lds16(at + (R + k) * row_bytes), z);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[j] = fma2(gp[j], mul2(x[j], r1), mul2(alpha, z[j]));
+      zv[k] = pack4p<DT>(z);
+      if (col && r + k < rows) st16(a.z + out + static_cast<int64_t>(k) * a.D, zv[k]);
+      unpack4p<DT>(zv[k], z);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fma2(z[j], z[j], s);
+      part[k] = col ? sum2(s) : 0.0f;
+    }
+    const float own2 = warp_sum4(part);
+    if ((lane & 7) == 0) red[1][team][lane >> 3][warp] = own2;
+    named_bar_sync(1 + team, team_threads);
+    const float root2 = rms_scale(team_sum4(red[1][team]), inv_d, a.eps);
+    f2_t h[INT8 ? R : 1][4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const f2_t r2 = splat2(__shfl_sync(kFull, root2, 8 * k));
+      f2_t(&o)[4] = h[INT8 ? k : 0];
+      f2_t z[4];
+      float amax = 0.0f;
+      unpack4p<DT>(zv[k], z);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[j] = fma2(ps[j], mul2(z[j], r2), sh[j]);
+        if (INT8) amax = max_abs_nan(amax, o[j]);
+      }
+      if (!INT8) {
+        if (col && r + k < rows) st16(a.h + out + static_cast<int64_t>(k) * a.D, pack4p<DT>(o));
+      } else {
+        const uint32_t m = warp_max_u32(col ? __float_as_uint(amax) : 0u);
+        if (lane == k) top = m;
+      }
+    }
+    if (INT8) {
+      if (lane < R) redu[team][lane][warp] = top;
+      named_bar_sync(1 + team, team_threads);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const uint32_t m = group_max_u32<16>(redu[team][k]);
+        const RowScale rs = row_scale(m);
+        if (col && r + k < rows) {
+          st8(a.q + out + static_cast<int64_t>(k) * a.D, codes8(h[INT8 ? k : 0], rs));
+          if (tid == 0) a.s[b * S + r0 + r + k] = scale_value(m);
+        }
+      }
+    }
+  }
+  // After a wait that gave up: copies in flight land before the block ends.
+  if (tid == 0 && !ok)
+    for (int i = asked > NS ? asked - NS : 0; i < asked; ++i) mbar_wait(bar0 + 8 * (i % NS), (i / NS) & 1);
+}
+
+// Rows of a block: one block a multiprocessor (148, whatever the device), of at
+// least `least` rows.
+static int64_t rows_of_block(int64_t B, int64_t S, int64_t least) {
+  const int64_t per_sample = B < 148 ? 148 / B : 1;
+  const int64_t c = (S + per_sample - 1) / per_sample;
+  return c > least ? c : least;
+}
+
+template <bool INT8>
+static cudaError_t launch_rows(const SandwichArgs& a, int64_t B, int64_t S, int dtype, cudaStream_t st) {
+  const int team = team_threads_of(a.D), teams = teams_of(a.D);
+  const int64_t chunk = rows_of_block(B, S, teams * kFwdRows);
+  const size_t smem = fwd_smem(a.D);
+  const dim3 grid(static_cast<unsigned>((S + chunk - 1) / chunk), static_cast<unsigned>(B)), block(team * teams);
+  auto kernel = dtype == kBf16 ? sandwich_rows_kernel<kBf16, INT8> : sandwich_rows_kernel<kFp16, INT8>;
+  const cudaError_t e = ensure_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kernel, grid, block, smem, st, a, S, static_cast<int>(chunk), team, teams);
+}
+
 template <int VPL, int GROUP, bool INT8>
 static cudaError_t launch_fwd_g(const SandwichArgs& a, int dtype, cudaStream_t st) {
   constexpr int BW = GROUP > 4 ? GROUP : 4;
@@ -208,8 +417,9 @@ static cudaError_t launch_fwd_g(const SandwichArgs& a, int dtype, cudaStream_t s
 }
 
 template <bool INT8>
-static cudaError_t launch_fwd(const SandwichArgs& a, int dtype, cudaStream_t st) {
+static cudaError_t launch_fwd(const SandwichArgs& a, int64_t B, int64_t S, int dtype, cudaStream_t st) {
   const int nv = a.D / 8;
+  if (a.rows >= kManyRows) return launch_rows<INT8>(a, B, S, dtype, st);
   if (nv <= 32) return launch_fwd_g<1, 1, INT8>(a, dtype, st);
   if (nv <= 64) return launch_fwd_g<2, 1, INT8>(a, dtype, st);
   if (nv <= 128) return launch_fwd_g<4, 1, INT8>(a, dtype, st);
@@ -239,13 +449,7 @@ struct SandwichBwdArgs {
 // row loop itself the kernel ran at 39% of memory speed, on their latency.
 constexpr int kBwdRows = 2;    // rows a team holds at once
 constexpr int kBwdStages = 3;  // of kBwdRows rows each
-constexpr int kBwdThreads = 512;
-static int bwd_team(int D) { return (D / 8 + 31) / 32 * 32; }
-static int bwd_teams(int D) {
-  const int t = kBwdThreads / bwd_team(D);
-  return t < 8 ? t : 8;
-}
-static size_t bwd_smem(int D) { return static_cast<size_t>(bwd_teams(D)) * kBwdStages * kBwdRows * 4 * D * 2; }
+static size_t bwd_smem(int D) { return static_cast<size_t>(teams_of(D)) * kBwdStages * kBwdRows * 4 * D * 2; }
 
 // Sums of eight values over the warp: lane l returns that of value l / 4.
 // Each step halves the values a lane carries, 9 exchanges for the 40 of eight
@@ -294,7 +498,7 @@ __device__ __forceinline__ float team_sum2(const float (*red)[16]) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kBwdThreads, 1) sandwich_bwd_kernel(const SandwichBwdArgs a, int team_threads, int teams) {
+__global__ void __launch_bounds__(kTeamThreads, 1) sandwich_bwd_kernel(const SandwichBwdArgs a, int team_threads, int teams) {
   constexpr int R = kBwdRows, NS = kBwdStages;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[8 * NS];
@@ -400,7 +604,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) sandwich_bwd_kernel(const Sand
     // Lanes of the first four values turn them into reciprocal roots; the
     // last two become the means of p zh.
     const float all = team_sum8(red1[team]);
-    const float root = rsqrtf(__fmaf_rn(all, inv_d, a.eps));
+    const float root = rms_scale(all, inv_d, a.eps);
     f2_t dm[R][4];  // dz gate post
     float rx[R], part[R];
 #pragma unroll
@@ -531,13 +735,9 @@ __global__ void __launch_bounds__(1024) sandwich_final_kernel(const SandwichFina
   }
 }
 
-// Rows of a backward block: one block a multiprocessor (148, whatever the
-// device: the sums' order follows from the sizes alone), of at least one pair
-// of rows for each team.
+// The order of the column sums follows from the sizes alone.
 static int64_t bwd_chunk(int64_t B, int64_t S, int64_t D) {
-  const int64_t per_sample = B < 148 ? 148 / B : 1;
-  const int64_t c = (S + per_sample - 1) / per_sample, least = bwd_teams(static_cast<int>(D)) * kBwdRows;
-  return c > least ? c : least;
+  return rows_of_block(B, S, teams_of(static_cast<int>(D)) * kBwdRows);
 }
 static bool check_sandwich(int64_t B, int64_t S, int64_t D, int dtype) {
   return check(B >= 0 && B <= 65535, "batch must be in [0, 65535]") &&
@@ -584,7 +784,7 @@ static int sandwich_fwd(const char* name, const void* x, const void* res, const 
   a.alpha = alpha;
   a.eps = eps;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return g.done(q != nullptr ? launch_fwd<true>(a, dtype, st) : launch_fwd<false>(a, dtype, st));
+  return g.done(q != nullptr ? launch_fwd<true>(a, B, S, dtype, st) : launch_fwd<false>(a, B, S, dtype, st));
 }
 
 extern "C" int afb_sandwich_norm(const void* x, const void* residual, const void* gate, const void* post_weight,
@@ -659,7 +859,7 @@ extern "C" int afb_sandwich_norm_bwd(const void* gh, const void* gz, const void*
   f.D = a.D;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(f.chunks), static_cast<unsigned>(batch));
-  const int team = bwd_team(a.D), teams = bwd_teams(a.D);
+  const int team = team_threads_of(a.D), teams = teams_of(a.D);
   const dim3 block(static_cast<unsigned>(team * teams));
   const size_t smem = bwd_smem(a.D);
   cudaError_t e = dtype == kBf16 ? ensure_smem(sandwich_bwd_kernel<kBf16>, smem) : ensure_smem(sandwich_bwd_kernel<kFp16>, smem);

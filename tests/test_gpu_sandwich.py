@@ -59,7 +59,8 @@ def _within(got, want, tol):
 
 
 SHAPES = [(1, 1, 8), (1, 1, 2048), (2, 3, 72), (3, 5, 256), (1, 7, 264), (2, 9, 512), (1, 4, 1024), (2, 33, 1032), (3, 11, 2048),
-          (1, 6, 2056), (2, 5, 4096), (1, 700, 640), (5, 1, 1152)]
+          (1, 6, 2056), (2, 5, 4096), (1, 700, 640), (5, 1, 1152), (3, 701, 264), (1, 2051, 2056), (2, 1030, 2048),
+          (1, 2049, 4096), (150, 15, 72)]
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
@@ -84,7 +85,8 @@ def test_forward_without_modulation(B, S, D, cuda_dev):
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
-@pytest.mark.parametrize("B,S,D", [(1, 1, 16), (2, 3, 144), (3, 5, 256), (2, 9, 512), (2, 33, 1040), (3, 11, 2048), (2, 5, 4096)])
+@pytest.mark.parametrize("B,S,D", [(1, 1, 16), (2, 3, 144), (3, 5, 256), (2, 9, 512), (2, 33, 1040), (3, 11, 2048), (2, 5, 4096), (3, 701, 272),
+                                   (2, 1030, 2048), (1, 2049, 4096)])
 def test_codes_of_the_output(B, S, D, dt, cuda_dev):
     c = _case(B, S, D, dt, 7 + D)
     q, s, z = _call(c, afb.sandwich_norm_int8)
