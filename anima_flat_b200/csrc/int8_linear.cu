@@ -131,6 +131,7 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
     // 32-bit sums of signed bytes, BN columns, 128 lanes.
     constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileN >> 4) << 24);
     const uint64_t desc0 = smem_desc(ring, 16, 1024);
+    const int total = first < a.tiles ? ((a.tiles - first - 1) / step + 1) * (kb1 - kb0) : 0;
     int it = 0, n = 0;
     bool ok = true;
     for (int tile = first; ok && tile < a.tiles; tile += step, ++n) {
@@ -150,7 +151,7 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
 #pragma unroll
           for (int k = 0; k < kKBlock / 32; ++k)
             mma_i8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, kb > kb0 || k > 0);
-          mma_commit(empty + 8 * st);
+          if (it + ST < total) mma_commit(empty + 8 * st);  // the last ones are not waited for
         }
         __syncwarp();
       }
@@ -250,6 +251,11 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
 // tokens, the first CTA issues the matrix instructions for both.  A stage then
 // costs a CTA (128 + BN / 2) rows from L2 for the work of 128 x BN: alone, with
 // 256 tokens, it asks for 96 bytes a clock, more than L2 gives.
+//
+// No arrival is under way to the other CTA's shared memory when a CTA leaves:
+// only those that someone waits for are made.  (With an arrival that nobody
+// waited for just before the last cluster barrier, a chain of several hundred
+// calls stopped.)
 __host__ __device__ constexpr int pair_stage_bytes(int bn) { return (kTileN + bn / 2) * kKBlock; }
 __host__ __device__ constexpr int pair_stages(int bn) { return bn >= 256 ? 6 : 8; }
 __host__ __device__ constexpr int pair_smem(int bn) { return pair_stages(bn) * pair_stage_bytes(bn) + 1024; }
@@ -281,6 +287,9 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
     }
     fence_mbar_init();
   }
+  // Both CTAs run, and their barriers are ready, before the pair allocates.
+  cluster_sync();
+  __syncwarp();
   if (warp == 1) tmem_alloc_pair(smem_addr(&tslot), lin_tmem(BN));
   tc_fence_before();
   cluster_sync();
@@ -323,6 +332,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
       constexpr uint32_t idesc =
           (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(2 * kTileN >> 4) << 24);
       const uint64_t desc0 = smem_desc(ring, 16, 1024);
+      const int total = first < a.tiles ? ((a.tiles - first - 1) / step + 1) * blocks : 0;
       int it = 0, n = 0;
       bool ok = true;
       for (int tile = first; ok && tile < a.tiles; tile += step, ++n) {
@@ -342,7 +352,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
 #pragma unroll
             for (int k = 0; k < kKBlock / 32; ++k)
               mma_i8_pair(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, kb > 0 || k > 0);
-            mma_commit_pair(empty + 8 * st);
+            if (it + ST < total) mma_commit_pair(empty + 8 * st);
           }
           __syncwarp();
         }
@@ -371,16 +381,18 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
       emit<DT>(a, trow + buf * BN, sm[buf], smem_addr(out[warp - 2][0]), n0 + quad * 32, m0, min(BN, a.M - m0), vn, b);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_at(acce0 + 8 * buf);
+      if (lane == 0 && tile + 2 * step < a.tiles) mbar_arrive_at(acce0 + 8 * buf);
     }
   }
   __syncwarp();
   tc_fence_before();
   cluster_sync();
   if (warp == 1) {
+    __syncwarp();
     tc_fence_after();
     tmem_free_pair(tmem, lin_tmem(BN));
   }
+  cluster_sync();  // neither CTA leaves while the pair frees
 }
 
 template <int BN, int DT>

@@ -164,8 +164,9 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
 #pragma unroll
         for (int k = 0; k < kTok / 16; ++k)  // 16 tokens: two groups of 8 rows
           mma_f16(tmem, da + k * (2048 >> 4), db + k * (16 * kRow >> 4), idesc, it > 0 || k > 0);
-        mma_commit(empty + 8 * st);
-        mma_commit(cempty + 8 * cs);
+        // the last ones are not waited for
+        if (it + R < nb) mma_commit(empty + 8 * st);
+        if (it + G < nb) mma_commit(cempty + 8 * cs);
       }
       __syncwarp();
     }
@@ -336,6 +337,9 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
     }
     fence_mbar_init();
   }
+  // Both CTAs run, and their barriers are ready, before the pair allocates.
+  cluster_sync();
+  __syncwarp();
   if (warp == 1) tmem_alloc_pair(smem_addr(&tslot), 2 * kPairCols);
   tc_fence_before();
   cluster_sync();
@@ -422,8 +426,10 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
 #pragma unroll
             for (int k = 0; k < kTok / 16; ++k)
               mma_f16_pair(tmem + buf * kPairCols, da + k * (2048 >> 4), db + k * (2048 >> 4), idesc, t > 0 || k > 0);
-            mma_commit_pair(dempty + 8 * ds);
-            mma_commit_pair(cempty + 8 * cs);
+            // No arrival is under way to the other CTA when a CTA leaves:
+            // only those that someone waits for are made.
+            if (it + kDRing < mine * blocks) mma_commit_pair(dempty + 8 * ds);
+            if (it + kCRing < mine * blocks) mma_commit_pair(cempty + 8 * cs);
           }
           __syncwarp();
         }
@@ -482,16 +488,18 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
                    [](int, int, uint32_t lo, uint32_t hi) { return pack2<DT>(__uint_as_float(lo), __uint_as_float(hi)); });
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_at(acce0 + 8 * buf);
+      if (lane == 0 && tile + 2 * step < tiles) mbar_arrive_at(acce0 + 8 * buf);
     }
   }
   __syncwarp();
   tc_fence_before();
   cluster_sync();
   if (warp == 1) {
+    __syncwarp();
     tc_fence_after();
     tmem_free_pair(tmem, 2 * kPairCols);
   }
+  cluster_sync();  // neither CTA leaves while the pair frees
 }
 
 template <int DT>

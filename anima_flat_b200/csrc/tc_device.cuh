@@ -105,7 +105,8 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
       "l"(m), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-// Both CTAs call these with one warp each.
+// Both CTAs call these with one warp each, between cluster barriers: the pair's
+// other CTA has to be running.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t slot, uint32_t cols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
