@@ -66,6 +66,7 @@ WORKSPACE_QUERIES: dict[str, tuple] = {
     "afb_head_norm_bwd_workspace": (_I, _I, _I, _I),
     "afb_rms_silu_bwd_workspace": (_I, _I),
     "afb_sandwich_norm_bwd_workspace": (_I, _I, _I),
+    "afb_int8_linear_x_workspace": (_I, _I, _I),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -204,7 +204,10 @@ __global__ void __launch_bounds__((GROUP > 4 ? GROUP : 4) * 32) sandwich_fwd_ker
 // threads take four rows at a time.  A thread owns 8 columns and keeps their
 // factors in registers; in the kernel above every row reads them again, 14 bytes
 // an element from L1 for 8 from memory.  Bulk copies keep the next rows coming.
-constexpr int64_t kManyRows = 2048;
+// From 2^19 elements on for rows of 1024 and more (256 x 2048: 4.0 us against 4.2
+// above, 1024 x 2048: 5.5 against 6.5; 128 x 2048: 4.0 and 4.0), from 2^22 for
+// shorter ones (8192 x 512: 8.6 against 9.1; 2048 x 512: 4.4 against 3.6).
+constexpr int64_t kManyWide = 1 << 19, kManyNarrow = 1 << 22;
 constexpr int kFwdRows = 4;
 constexpr int kFwdStages = 3;
 constexpr int kTeamThreads = 512;
@@ -419,7 +422,7 @@ static cudaError_t launch_fwd_g(const SandwichArgs& a, int dtype, cudaStream_t s
 template <bool INT8>
 static cudaError_t launch_fwd(const SandwichArgs& a, int64_t B, int64_t S, int dtype, cudaStream_t st) {
   const int nv = a.D / 8;
-  if (a.rows >= kManyRows) return launch_rows<INT8>(a, B, S, dtype, st);
+  if (a.rows * a.D >= (a.D >= 1024 ? kManyWide : kManyNarrow)) return launch_rows<INT8>(a, B, S, dtype, st);
   if (nv <= 32) return launch_fwd_g<1, 1, INT8>(a, dtype, st);
   if (nv <= 64) return launch_fwd_g<2, 1, INT8>(a, dtype, st);
   if (nv <= 128) return launch_fwd_g<4, 1, INT8>(a, dtype, st);

@@ -28,6 +28,7 @@ from typing import NamedTuple
 
 import torch
 
+from .._lib import load
 from .common import HALF_TYPES, _check_half, _check_same_device, _dense, _launch, _plain
 
 __all__ = [
@@ -79,11 +80,11 @@ def _quant_product(x, cols, wq, ws, bias):
     K, N = x.shape[-1], wq.shape[0]
     rows = x.numel() // K
     y = x.new_empty((*x.shape[:-1], N))
-    nbytes = rows * (K + 4)
-    work = x.new_empty(nbytes, dtype=I8)
+    nbytes = load().afb_int8_linear_x_workspace(rows, N, K)
+    work = x.new_empty(nbytes, dtype=I8) if nbytes else None
     _launch("afb_int8_linear_x", x, x.data_ptr(), None if cols is None else cols.data_ptr(), wq.data_ptr(),
             None if ws is None else ws.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), rows, N, K,
-            HALF_TYPES[x.dtype], work.data_ptr(), nbytes)
+            HALF_TYPES[x.dtype], None if work is None else work.data_ptr(), nbytes)
     return y
 
 

@@ -302,7 +302,9 @@ int afb_int8_linear(const void* q, const void* s, const void* w, const void* v, 
 
 /* The same from x [M, K] of `dtype`, or x * cols where cols [K] fp32 is not
  * NULL, quantised as by afb_rowquant_int8; v may be NULL (1).  K at most
- * 16384.  Workspace: M * (K + 4) bytes, 16-byte aligned, overwritten. */
+ * 16384.  Workspace: as many bytes as the query says (none for a few rows,
+ * which one launch takes), 16-byte aligned, overwritten. */
+size_t afb_int8_linear_x_workspace(int64_t M, int64_t N, int64_t K);
 int afb_int8_linear_x(const void* x, const void* cols, const void* w, const void* v,
                       const void* bias, void* y, int64_t M, int64_t N, int64_t K, int dtype,
                       void* workspace, size_t workspace_bytes, void* stream);
