@@ -11,8 +11,10 @@ Public functions mirror src/kernels/{adaln,fp8,rope,ctx_scale,rms}.py of the ref
 
 and, without a counterpart there:
 
-    rowquant_int8, quantize_weight_int8, int8_linear   (8-bit integer linear layers)
+    rowquant_int8, quantize_weight_int8, int8_linear, int8_linear_dx
+                                                  (8-bit integer linear layers)
     gelu_int8, gelu_int8_bwd, int8_wgrad, int8_restore (8-bit activation checkpoints)
+    int8_lora_mlp                                 (an MLP on these, with adapters)
     sandwich_norm, sandwich_norm_int8, sandwich_norm_bwd
                                                   (norms before and after a block)
 
@@ -28,11 +30,13 @@ from .kernels.int8 import (
     gelu_int8,
     gelu_int8_bwd,
     int8_linear,
+    int8_linear_dx,
     int8_restore,
     int8_wgrad,
     quantize_weight_int8,
     rowquant_int8,
 )
+from .kernels.int8_mlp import LoRA, int8_lora_mlp
 from .kernels.rms import add_rms_silu, rms_silu, shuffle_rms_silu
 from .kernels.rope import head_norm, qkv_norm_rope
 from .kernels.sandwich import sandwich_norm, sandwich_norm_bwd, sandwich_norm_int8
@@ -42,6 +46,7 @@ __all__ = [
     "FP8",
     "FP8_MAX",
     "Int8Weight",
+    "LoRA",
     "adaln",
     "adaln_fp8",
     "add_rms_silu",
@@ -51,6 +56,8 @@ __all__ = [
     "gelu_int8_bwd",
     "head_norm",
     "int8_linear",
+    "int8_linear_dx",
+    "int8_lora_mlp",
     "int8_restore",
     "int8_wgrad",
     "qkv_norm_rope",

@@ -51,7 +51,7 @@ SIGNATURES: dict[str, tuple] = {
     "afb_int8_restore": (_P, _P, _P, _I, _I, c_int, _P),
     "afb_int8_linear": (_P, _P, _P, _P, _P, _P, _I, _I, _I, c_int, _P),
     "afb_int8_linear_x": (_P, _P, _P, _P, _P, _P, _I, _I, _I, c_int, _P, ctypes.c_size_t, _P),
-    "afb_int8_wgrad": (_P, _P, _P, _P, _I, _I, _I, c_int, _P),
+    "afb_int8_wgrad": (_P, _P, _P, _P, _I, _I, _I, c_int, _P, ctypes.c_size_t, _P),
     "afb_sandwich_norm": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F, c_int, _P),
     "afb_sandwich_norm_int8": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F, c_int, _P),
     "afb_sandwich_norm_bwd": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I,
@@ -67,6 +67,7 @@ WORKSPACE_QUERIES: dict[str, tuple] = {
     "afb_rms_silu_bwd_workspace": (_I, _I),
     "afb_sandwich_norm_bwd_workspace": (_I, _I, _I),
     "afb_int8_linear_x_workspace": (_I, _I, _I),
+    "afb_int8_wgrad_workspace": (_I, _I, _I),
 }
 
 _lib: ctypes.CDLL | None = None

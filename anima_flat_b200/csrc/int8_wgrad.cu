@@ -24,6 +24,7 @@ struct WgradArgs {
   const float* s;  // [T]
   uint16_t* dw;    // [N, K]
   int T, N, K;
+  int ld;  // row length of dy, a multiple of 8
   int ktiles;
 };
 
@@ -274,7 +275,7 @@ static cudaError_t launch_wgrad(const void* dy, const void* q, WgradArgs a, int 
                                          : BN == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                     : CU_TENSOR_MAP_SWIZZLE_32B;
   if (e == cudaSuccess)
-    e = make_map(&gmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, swizzle, dy, a.N, a.T, static_cast<uint64_t>(a.N) * 2, wg_width(BN),
+    e = make_map(&gmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, swizzle, dy, a.ld, a.T, static_cast<uint64_t>(a.ld) * 2, wg_width(BN),
                  kTok);
   if (e == cudaSuccess) e = ensure_smem(int8_wgrad_kernel<BN, DT>, wg_smem(BN), true);
   if (e != cudaSuccess) return e;
@@ -507,8 +508,8 @@ static cudaError_t launch_wgrad_pair(const void* dy, const void* q, WgradArgs a,
   CUtensorMap qmap, gmap;
   cudaError_t e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, q, a.K, a.T, a.K, kCh, kTok);
   if (e == cudaSuccess)
-    e = make_map(&gmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B, dy, a.N, a.T,
-                 static_cast<uint64_t>(a.N) * 2, 64, kTok);
+    e = make_map(&gmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B, dy, a.ld, a.T,
+                 static_cast<uint64_t>(a.ld) * 2, 64, kTok);
   if (e == cudaSuccess) e = ensure_smem(int8_wgrad_pair_kernel<DT>, kPairSmem);
   if (e != cudaSuccess) return e;
   a.ktiles = (a.K + 2 * kCh - 1) / (2 * kCh);
@@ -547,28 +548,59 @@ static cudaError_t wgrad(const void* dy, const void* q, const WgradArgs& a, cuda
   }
 }
 
+// Rows of N elements into rows of ld: the copies of dy need rows of a multiple
+// of 16 bytes.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* x, uint16_t* y, int64_t total, DivU32 ld, int N) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t r = div_u32(ld, i), c = i - r * ld.d;
+  y[i] = c < N ? x[r * N + c] : 0;
+}
+
 cudaError_t read_status_int8_wgrad(int* status, bool clear) { return tu_status(status, clear); }
 
 }  // namespace afb
 
 using namespace afb;
 
+extern "C" size_t afb_int8_wgrad_workspace(int64_t rows, int64_t N, int64_t K) {
+  (void)K;
+  if (rows <= 0 || N <= 0 || N % 8 == 0) return 0;
+  if (rows > (1 << 30) || N > (1 << 20)) return SIZE_MAX;
+  return static_cast<size_t>(rows) * ((N + 7) / 8 * 8) * 2;
+}
+
 extern "C" int afb_int8_wgrad(const void* dy, const void* q, const void* s, void* dw, int64_t rows, int64_t N,
-                              int64_t K, int dtype, void* stream) {
+                              int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   ApiGuard g("afb_int8_wgrad");
   if (!check(rows >= 0 && rows <= (1 << 30), "rows must be in [0, 2^30]") ||
-      !check(N >= 8 && N % 8 == 0 && N <= (1 << 20), "N must be a multiple of 8 in [8, 2^20], got " + std::to_string(N)) ||
+      !check(N >= 1 && N <= (1 << 20), "N must be in [1, 2^20]") ||
       !check(K >= 16 && K % 16 == 0 && K <= (1 << 20), "K must be a multiple of 16 in [16, 2^20], got " + std::to_string(K)) ||
       !check_dtype(dtype) || !check_ptrs({dw}, {"dw"}))
     return g.fail();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (rows == 0) return g.done(cudaMemsetAsync(dw, 0, static_cast<size_t>(N) * K * 2, st));
-  if (!check_ptrs({dy, q}, {"dy", "q"}) || !check_ptr4(s, "s")) return g.fail();
+  if (!check_ptrs({dy, q}, {"dy", "q"}) || !check_ptr4(s, "s") ||
+      !check(workspace_bytes >= afb_int8_wgrad_workspace(rows, N, K), "workspace too small"))
+    return g.fail();
   WgradArgs a{};
   a.s = static_cast<const float*>(s);
   a.dw = static_cast<uint16_t*>(dw);
   a.T = static_cast<int>(rows);
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
+  a.ld = static_cast<int>((N + 7) / 8 * 8);
+  if (N % 8 != 0) {
+    if (!check_ptrs({workspace}, {"workspace"})) return g.fail();
+    const int64_t total = rows * a.ld;
+    if (!check((total + 255) / 256 <= INT64_C(0x7fffffff), "rows * N is too large")) return g.fail();
+    const cudaError_t e = launch_pdl(pad_rows_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0, st,
+                                     static_cast<const uint16_t*>(dy), static_cast<uint16_t*>(workspace), total,
+                                     make_divu32(a.ld), a.N);
+    if (e != cudaSuccess) return g.done(e);
+    dy = workspace;
+  }
   return g.done(dtype == kBf16 ? wgrad<kBf16>(dy, q, a, st) : wgrad<kFp16>(dy, q, a, st));
 }

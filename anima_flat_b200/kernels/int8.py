@@ -36,6 +36,7 @@ __all__ = [
     "gelu_int8",
     "gelu_int8_bwd",
     "int8_linear",
+    "int8_linear_dx",
     "int8_restore",
     "int8_wgrad",
     "quantize_weight_int8",
@@ -123,9 +124,12 @@ def _restore(q, s, dtype):
 
 def _wgrad(dy, q, s):
     N, K = dy.shape[-1], q.shape[-1]
+    rows = q.numel() // K
     dw = dy.new_empty((N, K))
-    _launch("afb_int8_wgrad", dy, dy.data_ptr(), q.data_ptr(), s.data_ptr(), dw.data_ptr(), q.numel() // K, N, K,
-            HALF_TYPES[dy.dtype])
+    nbytes = load().afb_int8_wgrad_workspace(rows, N, K) if N % 8 else 0
+    work = dy.new_empty(nbytes, dtype=I8) if nbytes else None
+    _launch("afb_int8_wgrad", dy, dy.data_ptr(), q.data_ptr(), s.data_ptr(), dw.data_ptr(), rows, N, K,
+            HALF_TYPES[dy.dtype], None if work is None else work.data_ptr(), nbytes)
     return dw
 
 
@@ -369,6 +373,37 @@ def int8_linear(
     return _LinearFn.apply(x, wq, ws, wqt, bias) if grad else _linear(x, wq, ws, wqt, bias)
 
 
+def int8_linear_dx(dy: torch.Tensor, weight: Int8Weight) -> torch.Tensor:
+    """Input gradient of ``int8_linear``: ``dy @ weight`` in 8-bit integers.
+
+    ``dy`` times the weight's scales is quantized per token and multiplied by
+    the transposed codes.  For a caller that writes its own backward pass;
+    ``int8_linear`` itself is differentiable.
+
+    Args:
+        dy: Gradient at the output, shape ``[..., N]`` bf16 or fp16, N a multiple of 16 up to 16384.
+        weight: The quantized weight ``[N, K]`` with its transposed codes.
+
+    Returns:
+        ``[..., K]``, dtype of ``dy``.
+
+    Raises:
+        ValueError: On tensors off CUDA, a weight without transposed codes, or
+            unsupported dtypes or shapes.
+    """
+    wq, ws, wqt = weight
+    if wqt is None:
+        raise ValueError("the input gradient needs quantize_weight_int8(w, backward=True)")
+    _check_same_device(dy, ws, wqt)
+    _check_half("dy", dy)
+    _check_cols("dy", dy)
+    N = dy.shape[-1]
+    if wqt.dtype != I8 or wqt.ndim != 2 or wqt.shape[1] != N or ws.dtype != F32 or ws.numel() != N:
+        raise ValueError(f"the transposed codes must be torch.int8 [K, {N}] with torch.float32 scales [{N}]")
+    dy, ws, wqt = _dense(dy), _dense(ws), _dense(wqt)
+    return _linear_bwd(dy, ws, wqt) if _plain(dy, ws, wqt) else _int8_linear_bwd(dy, ws, wqt)
+
+
 def gelu_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """GELU (the erf form) in 8 bits, with its input's 8-bit checkpoint.
 
@@ -443,9 +478,5 @@ def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tens
     _check_codes(q, s)
     if dy.shape[:-1] != q.shape[:-1] or not dy.shape[-1]:
         raise ValueError(f"dy and the codes must have the same tokens, got {list(dy.shape)} and {list(q.shape)}")
-    N = dy.shape[-1]
-    if N % 8:  # the kernel's copies of dy need rows of a multiple of 16 bytes
-        dy = torch.nn.functional.pad(dy, (0, -N % 8))
     dy, q, s = _dense(dy), _dense(q), s.contiguous()
-    dw = _wgrad(dy, q, s) if _plain(dy, q, s) else _int8_wgrad(dy, q, s)
-    return dw if dw.shape[0] == N else dw[:N]
+    return _wgrad(dy, q, s) if _plain(dy, q, s) else _int8_wgrad(dy, q, s)

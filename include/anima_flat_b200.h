@@ -309,11 +309,13 @@ int afb_int8_linear_x(const void* x, const void* cols, const void* w, const void
                       const void* bias, void* y, int64_t M, int64_t N, int64_t K, int dtype,
                       void* workspace, size_t workspace_bytes, void* stream);
 
-/* dw[n, k] = sum_t dy[t, n] q[t, k] s[t], summed in fp32.  dy [rows, N], N a
- * multiple of 8; q [rows, K], K a multiple of 16; s [rows]; dw [N, K] of
- * `dtype` (zero where rows = 0). */
+/* dw[n, k] = sum_t dy[t, n] q[t, k] s[t], summed in fp32 in an order that the
+ * sizes fix.  dy [rows, N]; q [rows, K], K a multiple of 16 up to 2^20;
+ * s [rows]; dw [N, K] of `dtype` (zero where rows = 0).  Workspace as the query
+ * says (none where N is a multiple of 8), 16-byte aligned, overwritten. */
+size_t afb_int8_wgrad_workspace(int64_t rows, int64_t N, int64_t K);
 int afb_int8_wgrad(const void* dy, const void* q, const void* s, void* dw, int64_t rows, int64_t N,
-                   int64_t K, int dtype, void* stream);
+                   int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ----------------------------------------------------------------------- */
 /* Norms before and after a block (no reference counterpart)                */

@@ -33,9 +33,10 @@ def _status(name, *args):
     ("afb_int8_linear", (FAKE, FAKE, FAKE, FAKE, None, FAKE, 4, 0, 32, 0, None), "N must be"),
     ("afb_int8_linear", (FAKE, FAKE, FAKE, FAKE, FAKE + 1, FAKE, 4, 8, 32, 0, None), "bias is not"),
     ("afb_int8_linear", (FAKE + 8, FAKE, FAKE, FAKE, None, FAKE, 4, 8, 32, 0, None), "q is not 16-byte aligned"),
-    ("afb_int8_wgrad", (FAKE, FAKE, FAKE, FAKE, 4, 12, 32, 0, None), "N must be"),
-    ("afb_int8_wgrad", (FAKE, FAKE, FAKE, FAKE, 4, 16, 40, 0, None), "K must be"),
-    ("afb_int8_wgrad", (FAKE, None, FAKE, FAKE, 4, 16, 32, 0, None), "q is null"),
+    ("afb_int8_wgrad", (FAKE, FAKE, FAKE, FAKE, 4, 0, 32, 0, None, 0, None), "N must be"),
+    ("afb_int8_wgrad", (FAKE, FAKE, FAKE, FAKE, 4, 12, 32, 0, FAKE, 127, None), "workspace too small"),
+    ("afb_int8_wgrad", (FAKE, FAKE, FAKE, FAKE, 4, 16, 40, 0, None, 0, None), "K must be"),
+    ("afb_int8_wgrad", (FAKE, None, FAKE, FAKE, 4, 16, 32, 0, None, 0, None), "q is null"),
     ("afb_sandwich_norm", (*([FAKE] * 9), 1, 4, 20, 1.0, 1e-6, 0, None), "dim must be"),
     ("afb_sandwich_norm", (*([FAKE] * 9), 1, 4, 4104, 1.0, 1e-6, 0, None), "dim must be"),
     ("afb_sandwich_norm", (*([FAKE] * 7), None, FAKE, 1, 4, 64, 1.0, 1e-6, 0, None), "h is null"),
