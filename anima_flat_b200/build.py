@@ -15,6 +15,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 if __package__:
@@ -27,18 +29,8 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
-NVCC_FLAGS = [
-    ARCH,
-    "-O3",
-    "-lineinfo",
-    "-std=c++17",
-    "--fmad=false",
-    "-Xcompiler",
-    "-fPIC,-O2",
-    "-shared",
-    "-cudart",
-    "static",
-]
+NVCC_FLAGS = [ARCH, "-O3", "-lineinfo", "-std=c++17", "--fmad=false", "-Xcompiler", "-fPIC,-O2"]
+LINK_FLAGS = ["-shared", "-Xcompiler", "-fPIC", "-cudart", "static"]
 
 
 def nvcc() -> str:
@@ -69,17 +61,25 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not _stale():
         return LIB_PATH
     LIB_DIR.mkdir(exist_ok=True)
+    def run(cmd: list[str]) -> None:
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stderr}")
+        if verbose and proc.stderr:
+            print(proc.stderr, file=sys.stderr)
+
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [nvcc(), *NVCC_FLAGS, f"-I{CSRC}", f"-I{INCLUDE}", "-o", str(tmp)]
-    cmd += [str(s) for s in sources()]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), file=sys.stderr)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stderr}")
-    if verbose and proc.stderr:
-        print(proc.stderr, file=sys.stderr)
+    flags = [*NVCC_FLAGS, *(["-Xptxas=-v"] if verbose else [])]
+    # one object per source, so that they compile side by side
+    with tempfile.TemporaryDirectory() as d, ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        objects = [str(Path(d) / f"{s.stem}.o") for s in sources()]
+        jobs = [pool.submit(run, [nvcc(), *flags, f"-I{CSRC}", f"-I{INCLUDE}", "-c", "-o", o, str(s)])
+                for s, o in zip(sources(), objects)]
+        for job in jobs:
+            job.result()
+        run([nvcc(), ARCH, *LINK_FLAGS, "-o", str(tmp), *objects])
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

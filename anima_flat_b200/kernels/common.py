@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from .._lib import call
+from .._lib import load
 
 BF16 = torch.bfloat16
 
@@ -93,11 +93,19 @@ def _plain(*ts: torch.Tensor | None) -> bool:
     return True
 
 
+_entries: dict[str, object] = {}
+
+
 def _launch(name: str, t: torch.Tensor, *args) -> None:
     """Call entry point `name` on the current stream of the device of `t`."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), name)
     device = t.get_device()
-    if device == torch.cuda.current_device():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        raise RuntimeError(f"{name} failed with status {rc}: {load().afb_last_error().decode(errors='replace')}")

@@ -80,7 +80,7 @@ def _quant_product(x, cols, wq, ws, bias):
     """Quantize x, or x * cols, and multiply: one call, its codes in a workspace."""
     K, N = x.shape[-1], wq.shape[0]
     rows = x.numel() // K
-    y = x.new_empty((*x.shape[:-1], N))
+    y = x.new_empty((rows, N) if x.ndim == 2 else (*x.shape[:-1], N))
     nbytes = load().afb_int8_linear_x_workspace(rows, N, K)
     work = x.new_empty(nbytes, dtype=I8) if nbytes else None
     _launch("afb_int8_linear_x", x, x.data_ptr(), None if cols is None else cols.data_ptr(), wq.data_ptr(),

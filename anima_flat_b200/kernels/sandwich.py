@@ -221,8 +221,10 @@ def sandwich_norm(x, residual, gate, post_weight, pre_weight, shift=None, scale=
     args = _args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
     if not _plain(*args[:7]):
         return _sandwich_norm(*args)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:7]):
-        return _SandwichFn.apply(*args)
+    if torch.is_grad_enabled():
+        for t in args[:7]:
+            if t is not None and t.requires_grad:
+                return _SandwichFn.apply(*args)
     return _fwd(*args)
 
 
