@@ -32,7 +32,7 @@ constexpr int kKBlock = 128;   // k of a stage: one swizzled row of 128 bytes
 constexpr int kThreads = 192;  // copy, matrix, four epilogue warps
 
 __host__ __device__ constexpr int lin_stage_bytes(int bn) { return (kTileN + bn) * kKBlock; }
-__host__ __device__ constexpr int lin_stages(int bn) { return bn >= 256 ? 4 : bn >= 128 ? 3 : bn >= 64 ? 4 : 5; }
+__host__ __device__ constexpr int lin_stages(int bn) { return bn >= 128 ? 3 : bn >= 64 ? 4 : 5; }
 __host__ __device__ constexpr int lin_smem(int bn) { return lin_stages(bn) * lin_stage_bytes(bn) + 1024; }
 __host__ __device__ constexpr int lin_tmem(int bn) { return 2 * bn < 32 ? 32 : 2 * bn; }
 
@@ -62,7 +62,7 @@ __device__ __forceinline__ void emit(const LinearArgs& a, uint32_t acc, const fl
 }
 
 template <int BN, int DT>
-__global__ void __launch_bounds__(kThreads, BN < 256 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, 2)
 int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap,
                    const LinearArgs a, int split) {
   constexpr int ST = lin_stages(BN), SB = lin_stage_bytes(BN);
@@ -256,15 +256,15 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
 // only those that someone waits for are made.  (With an arrival that nobody
 // waited for just before the last cluster barrier, a chain of several hundred
 // calls stopped.)
-__host__ __device__ constexpr int pair_stage_bytes(int bn) { return (kTileN + bn / 2) * kKBlock; }
-__host__ __device__ constexpr int pair_stages(int bn) { return bn >= 256 ? 6 : 8; }
-__host__ __device__ constexpr int pair_smem(int bn) { return pair_stages(bn) * pair_stage_bytes(bn) + 1024; }
+constexpr int kPairTok = 256;  // tokens of a pair's tile
+constexpr int kPairStages = 6, kPairStageBytes = (kTileN + kPairTok / 2) * kKBlock;
+constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024;
 
-template <int BN, int DT>
+template <int DT>
 __global__ void __launch_bounds__(kThreads, 1)
 int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap,
                         const LinearArgs a) {
-  constexpr int ST = pair_stages(BN), SB = pair_stage_bytes(BN);
+  constexpr int BN = kPairTok, ST = kPairStages, SB = kPairStageBytes;
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[2 * ST + 4];
   __shared__ __align__(8) float sm[2][BN];
@@ -395,19 +395,19 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
   cluster_sync();  // neither CTA leaves while the pair frees
 }
 
-template <int BN, int DT>
+template <int DT>
 static cudaError_t launch_pair(const void* q, const void* w, LinearArgs a, cudaStream_t st) {
   CUtensorMap wmap, qmap;
   const uint64_t K = static_cast<uint64_t>(a.K);
   cudaError_t e = make_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w, K, a.N, K, kKBlock, kTileN);
   if (e == cudaSuccess)
-    e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, q, K, a.M, K, kKBlock, BN / 2);
-  if (e == cudaSuccess) e = ensure_smem(int8_linear_pair_kernel<BN, DT>, pair_smem(BN));
+    e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, q, K, a.M, K, kKBlock, kPairTok / 2);
+  if (e == cudaSuccess) e = ensure_smem(int8_linear_pair_kernel<DT>, kPairSmem);
   if (e != cudaSuccess) return e;
   a.ntiles = (a.N + 2 * kTileN - 1) / (2 * kTileN);
-  a.tiles = a.ntiles * ((a.M + BN - 1) / BN);
+  a.tiles = a.ntiles * ((a.M + kPairTok - 1) / kPairTok);
   const int grid = 2 * std::min(a.tiles, device_info().sms / 2);
-  return launch_cluster(int8_linear_pair_kernel<BN, DT>, dim3(grid), dim3(kThreads), pair_smem(BN), 2, st, wmap, qmap, a);
+  return launch_cluster(int8_linear_pair_kernel<DT>, dim3(grid), dim3(kThreads), kPairSmem, 2, st, wmap, qmap, a);
 }
 
 template <int BN, int DT>
@@ -421,14 +421,15 @@ static cudaError_t launch_linear(const void* q, const void* w, LinearArgs a, int
   if (e != cudaSuccess) return e;
   a.ntiles = (a.N + kTileN - 1) / kTileN;
   a.tiles = a.ntiles * ((a.M + BN - 1) / BN);
-  const int grid = split > 1 ? a.tiles * split : std::min(a.tiles, device_info().sms * (BN < 256 ? 2 : 1));
+  const int grid = split > 1 ? a.tiles * split : std::min(a.tiles, device_info().sms * 2);
   return launch_cluster(int8_linear_kernel<BN, DT>, dim3(grid), dim3(kThreads), lin_smem(BN), split, st, wmap, qmap, a,
                         split);
 }
 
 // Tokens of a tile and parts along k.  Up to 128 tokens one tile holds them
-// all; above, the widest tile that still gives every multiprocessor one.  What
-// is left idle goes to parts of at least two k blocks.
+// all; above, 256 (pairs of CTAs) where tiles of 128 x 256 still give every
+// multiprocessor one, else 128.  What is left idle goes to parts of at least
+// two k blocks.
 static void linear_shape(int M, int N, int K, int sms, int* bn, int* split) {
   const int64_t nt = (N + kTileN - 1) / kTileN;
   auto tiles = [&](int b) { return nt * ((M + b - 1) / b); };
@@ -447,7 +448,7 @@ static cudaError_t linear(const void* q, const void* w, const LinearArgs& a, cud
   if (d.error != cudaSuccess) return d.error;
   int bn, split;
   linear_shape(a.M, a.N, a.K, d.sms, &bn, &split);
-  if (bn == 256) return launch_pair<256, DT>(q, w, a, st);
+  if (bn == 256) return launch_pair<DT>(q, w, a, st);
   switch (bn) {
     case 16: return launch_linear<16, DT>(q, w, a, split, st);
     case 32: return launch_linear<32, DT>(q, w, a, split, st);

@@ -18,8 +18,6 @@
 
 namespace afb {
 
-// Factors of the columns: a per-sample vector of the activations' type, or
-// null for a constant.
 struct SandwichArgs {
   const uint16_t* x;      // [B*S, D]
   const uint16_t* res;    // [B*S, D]
@@ -38,7 +36,8 @@ struct SandwichArgs {
   float alpha, eps;
 };
 
-// The same as pairs.
+// Eight factors of the columns as pairs: a per-sample vector of the activations'
+// type, or a constant where it is null.
 template <int DT>
 __device__ __forceinline__ void load4p(const uint16_t* p, float fallback, f2_t (&f)[4]) {
   if (p == nullptr) {
@@ -56,26 +55,6 @@ __device__ __forceinline__ void load4pf(const float* p, f2_t (&f)[4]) {
   f[1] = lo.y;
   f[2] = hi.x;
   f[3] = hi.y;
-}
-template <int DT>
-__device__ __forceinline__ void load8(const uint16_t* p, float fallback, float (&f)[8]) {
-  if (p == nullptr) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = fallback;
-    return;
-  }
-  const uint4 v = ld_keep(p);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const f2_t t = unpack2<DT>(word(v, j));
-    f[2 * j] = f2lo(t);
-    f[2 * j + 1] = f2hi(t);
-  }
-}
-__device__ __forceinline__ void load8f(const float* p, float (&f)[8]) {
-  const float4 lo = ld_keep_f4(p), hi = ld_keep_f4(p + 4);
-  f[0] = lo.x; f[1] = lo.y; f[2] = lo.z; f[3] = lo.w;
-  f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
 }
 template <int DT>
 __device__ __forceinline__ void unpack4p(const uint4 v, f2_t (&f)[4]) {
@@ -549,15 +528,15 @@ __global__ void __launch_bounds__(kTeamThreads, 1) sandwich_bwd_kernel(const San
 
   f2_t gw[4] = {}, pw[4] = {};  // gate * post, scale * pre
   if (col) {
-    float u[8], v[8];
-    load8<DT>(a.gate ? a.gate + b * a.D + e : nullptr, 1.0f, v);
-    load8f(a.post + e, u);
+    f2_t u[4];
+    load4pf(a.post + e, u);
+    load4p<DT>(a.gate ? a.gate + b * a.D + e : nullptr, 1.0f, gw);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) gw[j] = mul2(f2(u[2 * j], u[2 * j + 1]), f2(v[2 * j], v[2 * j + 1]));
-    load8<DT>(a.scale ? a.scale + b * a.D + e : nullptr, 1.0f, v);
-    load8f(a.pre + e, u);
+    for (int j = 0; j < 4; ++j) gw[j] = mul2(gw[j], u[j]);
+    load4pf(a.pre + e, u);
+    load4p<DT>(a.scale ? a.scale + b * a.D + e : nullptr, 1.0f, pw);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) pw[j] = mul2(f2(u[2 * j], u[2 * j + 1]), f2(v[2 * j], v[2 * j + 1]));
+    for (int j = 0; j < 4; ++j) pw[j] = mul2(pw[j], u[j]);
   }
   f2_t P[4] = {}, Q[4] = {}, G[4] = {};
   bool ok = true;

@@ -63,7 +63,13 @@ def _check_same_device(*ts: torch.Tensor | None) -> None:
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned: a copy only where `t` is not."""
+    """Contiguous and 16-byte aligned: a copy only where `t` is not.
+
+    While code is being compiled there is no address to look at; the registered
+    ops call this again on what they are given.
+    """
+    if torch.compiler.is_compiling():
+        return t.contiguous()
     if t.is_contiguous():
         return t if not t.data_ptr() & 15 else t.clone()
     return t.contiguous()

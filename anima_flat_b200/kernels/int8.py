@@ -150,7 +150,7 @@ class _LinearFn(torch.autograd.Function):
 # ----------------------------------------------------------------- custom ops --
 @torch.library.custom_op("anima_flat_b200::rowquant_int8", mutates_args=())
 def _rowquant_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return _quant(x)
+    return _quant(_dense(x))
 
 
 @_rowquant_int8.register_fake
@@ -163,7 +163,7 @@ def _int8_linear_codes(
     q: torch.Tensor, s: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias: torch.Tensor | None,
     dtype: torch.dtype,
 ) -> torch.Tensor:
-    return _product(q, s, wq, ws, bias, dtype)
+    return _product(_dense(q), s, _dense(wq), ws, bias, dtype)
 
 
 @_int8_linear_codes.register_fake
@@ -176,7 +176,7 @@ def _int8_linear(
     x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, wqt: torch.Tensor | None,
     bias: torch.Tensor | None,
 ) -> torch.Tensor:
-    return _linear(x, wq, ws, wqt, bias)
+    return _linear(_dense(x), _dense(wq), ws, wqt, bias)
 
 
 @_int8_linear.register_fake
@@ -186,7 +186,7 @@ def _(x, wq, ws, wqt, bias):
 
 @torch.library.custom_op("anima_flat_b200::int8_linear_bwd", mutates_args=())
 def _int8_linear_bwd(dy: torch.Tensor, ws: torch.Tensor, wqt: torch.Tensor) -> torch.Tensor:
-    return _linear_bwd(dy, ws, wqt)
+    return _linear_bwd(dy, _dense(ws), _dense(wqt))
 
 
 @_int8_linear_bwd.register_fake
@@ -211,7 +211,7 @@ torch.library.register_autograd(
 
 @torch.library.custom_op("anima_flat_b200::gelu_int8", mutates_args=())
 def _gelu_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _gelu(x)
+    return _gelu(_dense(x))
 
 
 @_gelu_int8.register_fake
@@ -223,7 +223,7 @@ def _(x):
 
 @torch.library.custom_op("anima_flat_b200::gelu_int8_bwd", mutates_args=())
 def _gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.Tensor:
-    return _gelu_bwd(dy, c, cs)
+    return _gelu_bwd(_dense(dy), _dense(c), cs)
 
 
 @_gelu_int8_bwd.register_fake
@@ -233,7 +233,7 @@ def _(dy, c, cs):
 
 @torch.library.custom_op("anima_flat_b200::int8_restore", mutates_args=())
 def _int8_restore(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    return _restore(q, s, dtype)
+    return _restore(_dense(q), s, dtype)
 
 
 @_int8_restore.register_fake
@@ -243,7 +243,7 @@ def _(q, s, dtype):
 
 @torch.library.custom_op("anima_flat_b200::int8_wgrad", mutates_args=())
 def _int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
-    return _wgrad(dy, q, s)
+    return _wgrad(_dense(dy), _dense(q), s)
 
 
 @_int8_wgrad.register_fake

@@ -23,6 +23,10 @@ __all__ = ["sandwich_norm", "sandwich_norm_bwd", "sandwich_norm_int8"]
 F32 = torch.float32
 
 
+def _dense_all(*ts: torch.Tensor | None):
+    return (None if t is None else _dense(t) for t in ts)
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -102,7 +106,7 @@ def _sandwich_norm(
     pre_weight: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None,
     residual_scale: float, eps: float,
 ) -> tuple[torch.Tensor, torch.Tensor]:
-    return _fwd(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
+    return _fwd(*_dense_all(x, residual, gate, post_weight, pre_weight, shift, scale), residual_scale, eps)
 
 
 @_sandwich_norm.register_fake
@@ -116,7 +120,7 @@ def _sandwich_norm_int8(
     pre_weight: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None,
     residual_scale: float, eps: float,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _fwd_int8(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
+    return _fwd_int8(*_dense_all(x, residual, gate, post_weight, pre_weight, shift, scale), residual_scale, eps)
 
 
 @_sandwich_norm_int8.register_fake
@@ -131,7 +135,7 @@ def _sandwich_norm_bwd(
     post_weight: torch.Tensor, pre_weight: torch.Tensor, scale: torch.Tensor | None,
     residual_scale: float, eps: float,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale, residual_scale, eps)
+    return _bwd(*_dense_all(gh, gz, z, x, gate, post_weight, pre_weight, scale), residual_scale, eps)
 
 
 @_sandwich_norm_bwd.register_fake
