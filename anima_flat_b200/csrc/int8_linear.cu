@@ -171,7 +171,7 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
       const bool nok = ch < a.N;
       const float vn = nok ? scale_of(a, ch) : 0.0f;
       const float b = nok && a.bias != nullptr ? load1<DT>(a.bias + ch) : 0.0f;
-      for (int i = et; i < BN; i += 128) sm[buf][i] = m0 + i < a.M ? __ldg(a.s + m0 + i) : 0.0f;
+      for (int i = et; i < BN; i += 128) sm[buf][i] = m0 + i < a.M ? __ldcg(a.s + m0 + i) : 0.0f;
       named_bar_sync(1, 128);
       ok = ok && mbar_wait(accf + 8 * buf, (n >> 1) & 1);
       if (!ok) continue;
@@ -373,7 +373,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
       const int ch = n0 + quad * 32 + lane;
       const float vn = ch < a.N ? scale_of(a, ch) : 0.0f;
       const float b = ch < a.N && a.bias != nullptr ? load1<DT>(a.bias + ch) : 0.0f;
-      for (int i = et; i < BN; i += 128) sm[buf][i] = m0 + i < a.M ? __ldg(a.s + m0 + i) : 0.0f;
+      for (int i = et; i < BN; i += 128) sm[buf][i] = m0 + i < a.M ? __ldcg(a.s + m0 + i) : 0.0f;
       named_bar_sync(1, 128);
       ok = ok && mbar_wait(accf + 8 * buf, (n >> 1) & 1);
       if (!ok) continue;

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(256) restore_kernel(const RestoreArgs a) {
     g[0] = ld_stream(a.dy + i * 16);
     g[1] = ld_stream(a.dy + i * 16 + 8);
   }
-  const float s = __ldg(a.s + div_u32(a.per_row, i));
+  const float s = __ldcg(a.s + div_u32(a.per_row, i));
   uint4 o[2];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {

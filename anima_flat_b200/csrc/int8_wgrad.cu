@@ -182,7 +182,7 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
     auto scale_at = [&](int it) {
       const int at = it + (lane >> 4) * G;
       const int t = (b0 + at) * kTok + ((lane >> 2) & 3) * 16 + w * 4 + (lane & 3);
-      return at < nb && t < a.T ? __ldg(a.s + t) : 0.0f;
+      return at < nb && t < a.T ? __ldcg(a.s + t) : 0.0f;
     };
     const int g = (warp - 2) >> 2;
     const uint32_t dst = ring + g * CB;
@@ -446,7 +446,7 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
     auto scale_at = [&](int it) {
       const int at = it + (lane >> 4) * kCRing;
       const int t = (at % blocks) * kTok + ((lane >> 2) & 3) * 16 + w * 4 + (lane & 3);
-      return at < total && t < a.T ? __ldg(a.s + t) : 0.0f;
+      return at < total && t < a.T ? __ldcg(a.s + t) : 0.0f;
     };
     float now = 0.0f, next = scale_at(g);
     int half = 0;

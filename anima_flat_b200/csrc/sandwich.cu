@@ -672,48 +672,69 @@ struct SandwichFinalArgs {
   int chunks, D;
 };
 
-// 32 columns a block; its 32 warps each sum every 32nd chunk, lane by column,
-// then each adds the warps' sums of one column.
+// 32 columns a block.  Its 32 warps form 1, 2 or 4 groups, which take the
+// samples in turn; a group's warps sum its chunks, lane by column, then every
+// warp adds its group's sums of some columns.  Five chunks are asked for at once
+// (148 blocks' by 32 warps): the kernel is one round trip to L2 long.
 template <int DT>
 __global__ void __launch_bounds__(1024) sandwich_final_kernel(const SandwichFinalArgs a) {
   __shared__ float red[3][32][33];
+  __shared__ float both[2][4][33];  // dpre and dpost of the groups
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int cl = blockIdx.x * 32 + lane, cw = blockIdx.x * 32 + warp;
-  const bool last = lane == 0 && cw < a.D;
+  const int groups = a.B >= 4 ? 4 : a.B >= 2 ? 2 : 1, per = 32 / groups;
+  const int g = warp / per, w = warp % per;
+  const int col0 = blockIdx.x * 32, cl = col0 + lane;
   pdl_wait();
   pdl_trigger();
-  const float post = last ? __ldg(a.post + cw) : 0.0f, pre = last ? __ldg(a.pre + cw) : 0.0f;
-  float dpost = 0.0f, dpre = 0.0f;
-  for (int64_t b = 0; b < a.B; ++b) {
-    const int64_t at = b * a.D + cw;
-    const float scale = last && a.scale ? load1<DT>(a.scale + at) : 1.0f;
-    const float gate = last && a.gate ? load1<DT>(a.gate + at) : 1.0f;
+  float dsum[2][4] = {};  // of the columns w, w + per, ... : dpre, dpost (lane 0)
+  for (int64_t b0 = 0; b0 < a.B; b0 += groups) {
+    const int64_t b = b0 + g;
     float s[3] = {};
-    if (cl < a.D) {
-#pragma unroll 4
-      for (int n = warp; n < a.chunks; n += 32) {
-        const float* p = a.part + (b * a.chunks + n) * 3 * a.D + cl;
+    if (cl < a.D && b < a.B) {
+      const float* base = a.part + b * a.chunks * 3 * a.D + cl;
+      for (int n0 = w; n0 < a.chunks; n0 += 5 * per) {
+        float v[5][3];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) s[i] += __ldg(p + static_cast<int64_t>(i) * a.D);
+        for (int u = 0; u < 5; ++u)
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            const int n = n0 + u * per;
+            v[u][i] = n < a.chunks ? __ldcg(base + (static_cast<int64_t>(n) * 3 + i) * a.D) : 0.0f;
+          }
+#pragma unroll
+        for (int u = 0; u < 5; ++u)
+#pragma unroll
+          for (int i = 0; i < 3; ++i) s[i] += v[u][i];
       }
     }
 #pragma unroll
     for (int i = 0; i < 3; ++i) red[i][warp][lane] = s[i];
     __syncthreads();
+    for (int k = 0; w + k * per < 32; ++k) {
+      const int c = w + k * per, at = col0 + c;
 #pragma unroll
-    for (int i = 0; i < 3; ++i) s[i] = warp_sum(red[i][lane][warp]);
-    __syncthreads();
-    if (last) {
-      dpre = __fmaf_rn(scale, s[0], dpre);
-      dpost = __fmaf_rn(gate, s[1], dpost);
-      if (a.dscale) a.dscale[at] = static_cast<uint16_t>(pack2<DT>(pre * s[0], 0.0f));
-      if (a.dgate) a.dgate[at] = static_cast<uint16_t>(pack2<DT>(post * s[1], 0.0f));
-      if (a.dshift) a.dshift[at] = static_cast<uint16_t>(pack2<DT>(s[2], 0.0f));
+      for (int i = 0; i < 3; ++i) s[i] = warp_sum(lane < per ? red[i][g * per + lane][c] : 0.0f);
+      if (lane == 0 && at < a.D && b < a.B) {
+        const int64_t o = b * a.D + at;
+        dsum[0][k] = __fmaf_rn(a.scale ? load1<DT>(a.scale + o) : 1.0f, s[0], dsum[0][k]);
+        dsum[1][k] = __fmaf_rn(a.gate ? load1<DT>(a.gate + o) : 1.0f, s[1], dsum[1][k]);
+        if (a.dscale) a.dscale[o] = static_cast<uint16_t>(pack2<DT>(__ldg(a.pre + at) * s[0], 0.0f));
+        if (a.dgate) a.dgate[o] = static_cast<uint16_t>(pack2<DT>(__ldg(a.post + at) * s[1], 0.0f));
+        if (a.dshift) a.dshift[o] = static_cast<uint16_t>(pack2<DT>(s[2], 0.0f));
+      }
     }
+    __syncthreads();
   }
-  if (last) {
-    a.dpost[cw] = dpost;
-    a.dpre[cw] = dpre;
+  if (lane == 0)
+    for (int k = 0; w + k * per < 32; ++k) {
+      both[0][g][w + k * per] = dsum[0][k];
+      both[1][g][w + k * per] = dsum[1][k];
+    }
+  __syncthreads();
+  if (warp < 2 && cl < a.D) {
+    float sum = 0.0f;
+    for (int i = 0; i < groups; ++i) sum += both[warp][i][lane];
+    (warp == 0 ? a.dpre : a.dpost)[cl] = sum;
   }
 }
 
