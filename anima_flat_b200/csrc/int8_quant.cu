@@ -19,13 +19,13 @@ struct QuantArgs {
   const float* cols;  // [K] or null: factors of the columns
   int8_t* q;          // [rows, K]: codes of x, x * cols or GELU(x)
   float* s;           // [rows]
-  int8_t* c;          // GELU only: codes of x
-  float* cs;          // GELU only
+  int8_t* c;          // GELU only: codes of x, and their scales
+  float* cs;
   int64_t rows;
   int K;
 };
 
-enum QuantMode { kPlain = 0, kCols = 1, kGelu = 2 };
+enum QuantMode { kPlain = 0, kCols = 1, kGelu = 2 };  // kGelu has its own kernel
 
 __host__ __device__ constexpr int quant_block_warps(int group) { return group > 4 ? group : 4; }
 
@@ -33,7 +33,7 @@ template <int CPL, int GROUP, int DT, int MODE>
 __global__ void __launch_bounds__(quant_block_warps(GROUP) * 32)
 rowquant_int8_kernel(const QuantArgs a) {
   constexpr int BW = quant_block_warps(GROUP);
-  __shared__ uint32_t red[2][BW];
+  __shared__ uint32_t red[BW];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -53,7 +53,7 @@ rowquant_int8_kernel(const QuantArgs a) {
     xv[c][1] = ok ? ld_stream(a.x + base + e + 8) : make_uint4(0, 0, 0, 0);
   }
   f2_t y[CPL][2][4];
-  float amax[2] = {0.0f, 0.0f};  // of y; of x where GELU keeps both
+  float amax = 0.0f;
 #pragma unroll
   for (int c = 0; c < CPL; ++c) {
     const int e = (t + 32 * GROUP * c) * 16;
@@ -70,83 +70,161 @@ rowquant_int8_kernel(const QuantArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const f2_t v = unpack2<DT>(word(xv[c][h], j));
-        if (MODE == kGelu) amax[1] = max_abs_nan(amax[1], v);
-        y[c][h][j] = MODE == kGelu ? fast_gelu2(v) : MODE == kCols ? mul2(v, f2(f[2 * j], f[2 * j + 1])) : v;
-        amax[0] = max_abs_nan(amax[0], y[c][h][j]);
+        y[c][h][j] = MODE == kCols ? mul2(v, f2(f[2 * j], f[2 * j + 1])) : v;
+        amax = max_abs_nan(amax, y[c][h][j]);
       }
     }
   }
-  uint32_t top[2];
-#pragma unroll
-  for (int n = 0; n < (MODE == kGelu ? 2 : 1); ++n) top[n] = warp_max_u32(__float_as_uint(amax[n]));
+  uint32_t top = warp_max_u32(__float_as_uint(amax));
   if (GROUP > 1) {
-    if (lane == 0) {
-      red[0][warp] = top[0];
-      if (MODE == kGelu) red[1][warp] = top[1];
-    }
+    if (lane == 0) red[warp] = top;
     __syncthreads();
-    const int w0 = (warp / GROUP) * GROUP;
-    top[0] = group_max_u32<GROUP>(&red[0][w0]);
-    if (MODE == kGelu) top[1] = group_max_u32<GROUP>(&red[1][w0]);
+    top = group_max_u32<GROUP>(&red[(warp / GROUP) * GROUP]);
   }
   if (!row_ok) return;
-  const RowScale r = row_scale(top[0]);
-  if (t == 0) a.s[row] = scale_value(top[0]);
+  const RowScale r = row_scale(top);
+  if (t == 0) a.s[row] = scale_value(top);
 #pragma unroll
   for (int c = 0; c < CPL; ++c) {
     const int e = (t + 32 * GROUP * c) * 16;
     if (e >= K) continue;
-    const uint2 lo = codes8<MODE != kGelu>(y[c][0], r), hi = codes8<MODE != kGelu>(y[c][1], r);
+    const uint2 lo = codes8(y[c][0], r), hi = codes8(y[c][1], r);
     st16(a.q + base + e, make_uint4(lo.x, lo.y, hi.x, hi.y));
-  }
-  if (MODE == kGelu) {
-    const RowScale rx = row_scale(top[1]);
-    if (t == 0) a.cs[row] = scale_value(top[1]);
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      const int e = (t + 32 * GROUP * c) * 16;
-      if (e >= K) continue;
-      uint2 o[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f2_t v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = unpack2<DT>(word(xv[c][h], j));
-        o[h] = codes8(v, rx);
-      }
-      st16(a.c + base + e, make_uint4(o[0].x, o[0].y, o[1].x, o[1].y));
-    }
   }
 }
 
-// The smallest power-of-two group whose threads hold at most `per` chunks of 16
-// each; two above 8192 columns.  Measured at K = 8192: the plain forms take
-// 31.8 us for 8192 rows with two chunks a thread and 40.5 with one, which waits
-// on twice the warps; GELU, bound by its arithmetic, 87.9 and 77.1, since fewer
-// registers keep more rows on a multiprocessor.
-static bool quant_shape(int64_t K, int per, int* group, int* cpl) {
+// GELU and its input's codes.  |GELU| is at most 0.17 below zero and increases
+// above it, so from x = 0.34 on the row's largest |GELU| is that of its largest
+// x: the row's scale is known before any GELU is formed, and each is formed and
+// coded on the spot, where holding them until a maximum is known took 57
+// registers a thread.  A row without such an x forms them twice.
+template <int CPL, int GROUP, int DT>
+__global__ void __launch_bounds__(quant_block_warps(GROUP) * 32)
+gelu_int8_kernel(const QuantArgs a) {
+  constexpr int BW = quant_block_warps(GROUP);
+  __shared__ uint32_t red[3][BW];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const int t = (warp % GROUP) * 32 + lane, w0 = (warp / GROUP) * GROUP;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (BW / GROUP) + warp / GROUP;
+  const bool row_ok = row < a.rows;
+  const int K = a.K;
+  const int64_t base = (row_ok ? row : 0) * K;
+  // The group's maximum; its warps alone meet.
+  auto group_max = [&](float v, int buf) {
+    uint32_t m = warp_max_u32(__float_as_uint(v));
+    if (GROUP > 1) {
+      if (lane == 0) red[buf][warp] = m;
+      named_bar_sync(1 + warp / GROUP, GROUP * 32);
+      m = group_max_u32<GROUP>(&red[buf][w0]);
+    }
+    return m;
+  };
+
+  uint4 xv[CPL][2];
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) {
+    const int e = (t + 32 * GROUP * c) * 16;
+    const bool ok = row_ok && e < K;
+    xv[c][0] = ok ? ld_stream(a.x + base + e) : make_uint4(0, 0, 0, 0);
+    xv[c][1] = ok ? ld_stream(a.x + base + e + 8) : make_uint4(0, 0, 0, 0);
+  }
+  float amax = 0.0f, pmax = 0.0f;  // of |x|, and of x above zero
+#pragma unroll
+  for (int c = 0; c < CPL; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const f2_t v = unpack2<DT>(word(xv[c][j >> 2], j & 3));
+      amax = max_abs_nan(amax, v);
+      pmax = fmaxf(pmax, fmaxf(f2lo(v), f2hi(v)));
+    }
+  const uint32_t top = group_max(amax, 0);
+  const float most = __uint_as_float(group_max(pmax, 1));
+  uint32_t gtop = __float_as_uint(f2lo(fast_gelu2(splat2(most))));
+  if (top >= 0x7f800000u) {
+    gtop = top;
+  } else if (most < 0.34f) {
+    float g = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CPL; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g = max_abs_nan(g, fast_gelu2(unpack2<DT>(word(xv[c][j >> 2], j & 3))));
+    gtop = group_max(g, 2);
+  }
+  if (!row_ok) return;
+  const RowScale rg = row_scale(gtop), rx = row_scale(top);
+  if (t == 0) {
+    a.s[row] = scale_value(gtop);
+    a.cs[row] = scale_value(top);
+  }
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) {
+    const int e = (t + 32 * GROUP * c) * 16;
+    if (e >= K) continue;
+    uint2 q[2], x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f2_t v[4], g[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = unpack2<DT>(word(xv[c][h], j));
+        g[j] = fast_gelu2(v[j]);
+      }
+      q[h] = codes8<false>(g, rg);
+      x[h] = codes8(v, rx);
+    }
+    st16(a.q + base + e, make_uint4(q[0].x, q[0].y, q[1].x, q[1].y));
+    st16(a.c + base + e, make_uint4(x[0].x, x[0].y, x[1].x, x[1].y));
+  }
+}
+
+// Warps of a row's group and chunks of 16 a thread.  The plain forms take two
+// chunks a thread (one where 32 threads hold the row): 8192 rows of 8192 take
+// 31.8 us so, 40.5 with one, which waits on twice the warps.  GELU takes one up
+// to 8 warps (4096 x 2048: 10.0 us, 12.3 with two) and two from there on
+// (8192 x 8192: 61.9 us with 8 warps, 75.9 with 16).
+template <int MODE>
+static bool quant_shape(int64_t K, int* group, int* cpl) {
   const int64_t chunks = K / 16;
   int g = 1;
-  while (g < 16 && chunks > 32 * per * g) g <<= 1;
+  if (MODE == kGelu)
+    while (g < 8 && chunks > 32 * g) g <<= 1;
+  while (g < 16 && chunks > 64 * g) g <<= 1;
   *group = g;
   *cpl = chunks > 32 * g ? 2 : 1;
   return K >= 16 && K % 16 == 0 && chunks <= 64 * g;
 }
+// Which of them quant_shape gives: one chunk with one warp, or for GELU with up
+// to 8; two with any number, for GELU with 8 and 16.
+template <int MODE, int GROUP, int CPL>
+constexpr bool quant_used() {
+  if (MODE == kGelu) return CPL == 1 ? GROUP <= 8 : GROUP >= 8;
+  return CPL == 2 || GROUP == 1;
+}
 
+template <int CPL, int GROUP, int DT, int MODE>
+static auto quant_kernel() {
+  if constexpr (MODE == kGelu) return gelu_int8_kernel<CPL, GROUP, DT>;
+  else return rowquant_int8_kernel<CPL, GROUP, DT, MODE>;
+}
 template <int GROUP, int DT, int MODE>
 static cudaError_t launch_quant_g(const QuantArgs& a, int cpl, cudaStream_t st) {
   constexpr int BW = quant_block_warps(GROUP);
   const int64_t per = BW / GROUP;
   const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per)), block(BW * 32);
-  if constexpr (GROUP == 16 || MODE != kGelu)
-    if (cpl == 2) return launch_pdl(rowquant_int8_kernel<2, GROUP, DT, MODE>, grid, block, 0, st, a);
-  return launch_pdl(rowquant_int8_kernel<1, GROUP, DT, MODE>, grid, block, 0, st, a);
+  if constexpr (quant_used<MODE, GROUP, 2>())
+    if (cpl == 2) return launch_pdl(quant_kernel<2, GROUP, DT, MODE>(), grid, block, 0, st, a);
+  if constexpr (quant_used<MODE, GROUP, 1>())
+    if (cpl == 1) return launch_pdl(quant_kernel<1, GROUP, DT, MODE>(), grid, block, 0, st, a);
+  return cudaErrorInvalidValue;
 }
 
 template <int DT, int MODE>
 static cudaError_t launch_quant(const QuantArgs& a, cudaStream_t st) {
   int group = 0, cpl = 0;
-  if (!quant_shape(a.K, MODE == kGelu ? 1 : 2, &group, &cpl)) return cudaErrorInvalidValue;
+  if (!quant_shape<MODE>(a.K, &group, &cpl)) return cudaErrorInvalidValue;
   switch (group) {
     case 1: return launch_quant_g<1, DT, MODE>(a, cpl, st);
     case 2: return launch_quant_g<2, DT, MODE>(a, cpl, st);
@@ -236,7 +314,7 @@ static cudaError_t launch_restore(const RestoreArgs& a, int dtype, cudaStream_t 
 static bool check_quant(int64_t rows, int64_t K, int dtype) {
   int group = 0, cpl = 0;
   return check(rows >= 0 && rows <= INT64_C(0x7fffffff), "rows must be in [0, 2^31)") &&
-         check(quant_shape(K, 2, &group, &cpl),
+         check(quant_shape<kPlain>(K, &group, &cpl),
                "K must be a multiple of 16 in [16, 16384], got " + std::to_string(K)) &&
          check_dtype(dtype);
 }

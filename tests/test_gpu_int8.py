@@ -267,6 +267,29 @@ def test_gelu_codes_and_checkpoint(shape, dt, cuda_dev):
     _within(q.view(-1, K).double() * s.double(), y, 0.5001 * s.double() + 2 * err)
 
 
+@pytest.mark.parametrize("K", [16, 512, 528, 1024, 2048, 4096, 8192, 8208, 16384])
+def test_gelu_rows_without_a_large_positive_value(K, cuda_dev):
+    """Rows whose largest |GELU| is not that of their largest input, beside rows where it is."""
+    g = _gen(K)
+    x = 2.0 * torch.randn(11, K, generator=g, device=cuda_dev)
+    x[1] = -x[1].abs()
+    x[3] *= 0.05
+    x[4] = 0
+    x[6] = -x[6].abs() * 0.01
+    x[7] = -20.0
+    x[9, : K - 1] = -x[9, : K - 1].abs()
+    x[9, K - 1] = 0.2
+    x = x.to(BF)
+    q, s, c, cs = afb.gelu_int8(x)
+    cq, csc = afb.rowquant_int8(x)
+    assert torch.equal(c, cq) and torch.equal(cs, csc)
+    y = _gelu64(x.double())
+    top = y.abs().amax(1, keepdim=True)
+    err = 2.0**-20 + 2.0**-12 * y.abs()
+    _within(s, top.clamp_min(1e-30) / 127.0, (2.0**-20 + 2.0**-12 * top) / 127.0 + 2.0**-23 * top / 127.0)
+    _within(q.double() * s.double(), y, 0.5001 * s.double() + 2 * err)
+
+
 @pytest.mark.parametrize("dt", [BF, HF])
 @pytest.mark.parametrize("shape", [(1, 16), (3, 48), (2, 5, 528), (77, 2048), (9, 8192), (3, 16384)])
 def test_gelu_backward_from_codes(shape, dt, cuda_dev):
