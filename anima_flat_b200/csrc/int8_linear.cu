@@ -256,15 +256,16 @@ int8_linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_consta
 // only those that someone waits for are made.  (With an arrival that nobody
 // waited for just before the last cluster barrier, a chain of several hundred
 // calls stopped.)
-constexpr int kPairTok = 256;  // tokens of a pair's tile
+constexpr int kPairTok = 256;  // tokens of a pair's widest tile
 constexpr int kPairStages = 6, kPairStageBytes = (kTileN + kPairTok / 2) * kKBlock;
 constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024;
 
 template <int DT>
 __global__ void __launch_bounds__(kThreads, 1)
 int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap,
-                        const LinearArgs a) {
-  constexpr int BN = kPairTok, ST = kPairStages, SB = kPairStageBytes;
+                        const LinearArgs a, int bn) {
+  constexpr int BN = kPairTok, ST = kPairStages, SB = kPairStageBytes;  // the widest tile's
+  const uint32_t stage_bytes = (kTileN + bn / 2) * kKBlock;
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[2 * ST + 4];
   __shared__ __align__(8) float sm[2][BN];
@@ -307,7 +308,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
     int it = 0, sent = 0;
     bool ok = true;
     for (int tile = first; ok && tile < a.tiles; tile += step) {
-      const int n0 = channel0(tile), m0 = (tile / a.ntiles) * BN + rank * (BN / 2);
+      const int n0 = channel0(tile), m0 = (tile / a.ntiles) * bn + rank * (bn / 2);
       for (int kb = 0; kb < blocks; ++kb, ++it) {
         const int st = it % ST;
         if (it >= ST && !mbar_wait(empty + 8 * st, ((it / ST) - 1) & 1)) {
@@ -315,7 +316,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
           break;
         }
         if (elect_one()) {
-          if (rank == 0) mbar_arrive_expect_tx(full + 8 * st, 2 * SB);
+          if (rank == 0) mbar_arrive_expect_tx(full + 8 * st, 2 * stage_bytes);
           tma_load_pair(ring + st * SB, &wmap, kb * kKBlock, n0, full0 + 8 * st);
           tma_load_pair(ring + st * SB + kTileN * kKBlock, &qmap, kb * kKBlock, m0, full0 + 8 * st);
         }
@@ -329,8 +330,8 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
       for (int i = sent > ST ? sent - ST : 0; i < sent; ++i) mbar_wait(full + 8 * (i % ST), (i / ST) & 1);
   } else if (warp == 1) {
     if (rank == 0) {
-      constexpr uint32_t idesc =
-          (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (uint32_t(2 * kTileN >> 4) << 24);
+      const uint32_t idesc =
+          (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(bn >> 3) << 17) | (uint32_t(2 * kTileN >> 4) << 24);
       const uint64_t desc0 = smem_desc(ring, 16, 1024);
       const int total = first < a.tiles ? ((a.tiles - first - 1) / step + 1) * blocks : 0;
       int it = 0, n = 0;
@@ -369,16 +370,16 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
     bool ok = true;
     for (int tile = first; tile < a.tiles; tile += step, ++n) {
       const int buf = n & 1;
-      const int n0 = channel0(tile), m0 = (tile / a.ntiles) * BN;
+      const int n0 = channel0(tile), m0 = (tile / a.ntiles) * bn;
       const int ch = n0 + quad * 32 + lane;
       const float vn = ch < a.N ? scale_of(a, ch) : 0.0f;
       const float b = ch < a.N && a.bias != nullptr ? load1<DT>(a.bias + ch) : 0.0f;
-      for (int i = et; i < BN; i += 128) sm[buf][i] = m0 + i < a.M ? __ldcg(a.s + m0 + i) : 0.0f;
+      for (int i = et; i < bn; i += 128) sm[buf][i] = m0 + i < a.M ? __ldcg(a.s + m0 + i) : 0.0f;
       named_bar_sync(1, 128);
       ok = ok && mbar_wait(accf + 8 * buf, (n >> 1) & 1);
       if (!ok) continue;
       tc_fence_after();
-      emit<DT>(a, trow + buf * BN, sm[buf], smem_addr(out[warp - 2][0]), n0 + quad * 32, m0, min(BN, a.M - m0), vn, b);
+      emit<DT>(a, trow + buf * BN, sm[buf], smem_addr(out[warp - 2][0]), n0 + quad * 32, m0, min(bn, a.M - m0), vn, b);
       tc_fence_before();
       __syncwarp();
       if (lane == 0 && tile + 2 * step < a.tiles) mbar_arrive_at(acce0 + 8 * buf);
@@ -396,18 +397,18 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_c
 }
 
 template <int DT>
-static cudaError_t launch_pair(const void* q, const void* w, LinearArgs a, cudaStream_t st) {
+static cudaError_t launch_pair(const void* q, const void* w, LinearArgs a, int bn, cudaStream_t st) {
   CUtensorMap wmap, qmap;
   const uint64_t K = static_cast<uint64_t>(a.K);
   cudaError_t e = make_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w, K, a.N, K, kKBlock, kTileN);
   if (e == cudaSuccess)
-    e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, q, K, a.M, K, kKBlock, kPairTok / 2);
+    e = make_map(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, q, K, a.M, K, kKBlock, bn / 2);
   if (e == cudaSuccess) e = ensure_smem(int8_linear_pair_kernel<DT>, kPairSmem);
   if (e != cudaSuccess) return e;
   a.ntiles = (a.N + 2 * kTileN - 1) / (2 * kTileN);
-  a.tiles = a.ntiles * ((a.M + kPairTok - 1) / kPairTok);
+  a.tiles = a.ntiles * ((a.M + bn - 1) / bn);
   const int grid = 2 * std::min(a.tiles, device_info().sms / 2);
-  return launch_cluster(int8_linear_pair_kernel<DT>, dim3(grid), dim3(kThreads), kPairSmem, 2, st, wmap, qmap, a);
+  return launch_cluster(int8_linear_pair_kernel<DT>, dim3(grid), dim3(kThreads), kPairSmem, 2, st, wmap, qmap, a, bn);
 }
 
 template <int BN, int DT>
@@ -442,13 +443,33 @@ static void linear_shape(int M, int N, int K, int sms, int* bn, int* split) {
   *split = s;
 }
 
+// Tokens of a pair's tile: of 256, 224, 192 and 160 the one whose whole rounds
+// of tiles take least, by the cycles of a block of k: 2 for a token's matrix
+// instructions, or what L2 takes for its (128 + bn / 2) rows of 128 bytes at 66
+// bytes a cycle.  1024 x 2048 -> 6144, 1.3 rounds of 256 or 1.9 of 192: 15.9 us
+// and 13.8.
+static int pair_tokens(int M, int N, int pairs) {
+  const int64_t nt = (N + 2 * kTileN - 1) / (2 * kTileN);
+  int best = kPairTok;
+  int64_t least = INT64_MAX;
+  for (int bn = kPairTok; bn >= 160; bn -= 32) {
+    const int64_t rounds = (nt * ((M + bn - 1) / bn) + pairs - 1) / pairs;
+    const int64_t cost = rounds * std::max(2 * bn, (kTileN + bn / 2) * kKBlock / 66);
+    if (cost < least) {
+      least = cost;
+      best = bn;
+    }
+  }
+  return best;
+}
+
 template <int DT>
 static cudaError_t linear(const void* q, const void* w, const LinearArgs& a, cudaStream_t st) {
   const DeviceInfo& d = device_info();
   if (d.error != cudaSuccess) return d.error;
   int bn, split;
   linear_shape(a.M, a.N, a.K, d.sms, &bn, &split);
-  if (bn == 256) return launch_pair<DT>(q, w, a, st);
+  if (bn == 256) return launch_pair<DT>(q, w, a, pair_tokens(a.M, a.N, d.sms / 2), st);
   switch (bn) {
     case 16: return launch_linear<16, DT>(q, w, a, split, st);
     case 32: return launch_linear<32, DT>(q, w, a, split, st);

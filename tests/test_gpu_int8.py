@@ -139,7 +139,8 @@ def _check_linear(y, q64, s, w, b, dt):
 LINEAR = [(1, 16, 16), (6, 300, 4096), (7, 33, 8192), (1, 4097, 16384), (2, 5000, 144), (8, 2049, 4096), (1, 1, 16), (1, 2047, 2048), (2, 130, 144), (3, 7, 4112), (4, 96, 8192), (5, 128, 2064),
           (8, 257, 1024), (9, 64, 1040), (16, 127, 2048), (17, 129, 528), (33, 640, 256), (64, 63, 4096), (65, 1000, 272),
           (77, 2047, 1024), (128, 128, 128), (129, 255, 2032), (200, 256, 16384), (257, 513, 1040), (512, 2048, 2048),
-          (1000, 33, 2048), (1537, 1030, 2064), (4096, 2048, 512), (4099, 3001, 1040)]
+          (1000, 33, 2048), (1537, 1030, 2064), (4096, 2048, 512), (4099, 3001, 1040), (1024, 6144, 272), (1000, 8192, 144),
+          (2304, 5000, 528)]
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
