@@ -236,14 +236,24 @@ __device__ __forceinline__ void emit_columns(uint32_t acc, uint32_t st0, int col
         if (c + row < cols && at < ld) st16(y + static_cast<int64_t>(c + row) * ld + at, w);
       }
     } else {
-#pragma unroll 4
-      for (int row = 0; row < 16; ++row) {
-        uint16_t w;
-        asm volatile("ld.shared.u16 %0, [%1];"
-                     : "=h"(w)
-                     : "r"(stage + row * 64 + (((lane >> 3) ^ (row >> 1)) & 3) * 16 + (lane & 7) * 2)
-                     : "memory");
-        if (c + row < cols && run + lane < ld) y[static_cast<int64_t>(c + row) * ld + run + lane] = w;
+      // a channel a lane; eight rows are read before the first is written
+#pragma unroll
+      for (int r0 = 0; r0 < 16; r0 += 8) {
+        uint16_t w[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int row = r0 + r;
+          asm volatile("ld.shared.u16 %0, [%1];"
+                       : "=h"(w[r])
+                       : "r"(stage + row * 64 + (((lane >> 3) ^ (row >> 1)) & 3) * 16 + (lane & 7) * 2)
+                       : "memory");
+        }
+        if (run + lane < ld) {
+          uint16_t* at = y + static_cast<int64_t>(c + r0) * ld + run + lane;
+#pragma unroll
+          for (int r = 0; r < 8; ++r, at += ld)
+            if (c + r0 + r < cols) *at = w[r];
+        }
       }
     }
   }
