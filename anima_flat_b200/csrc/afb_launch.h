@@ -134,12 +134,12 @@ inline bool check_ptrs(std::initializer_list<const void*> ps, std::initializer_l
   return true;
 }
 inline bool check_ptr8(const void* p, const char* nm) {
-  return check(p != nullptr, std::string(nm) + " is null") &&
-         check(aligned(p, 8), std::string(nm) + " is not 8-byte aligned");
+  if (p == nullptr) return check(false, std::string(nm) + " is null");
+  return aligned(p, 8) || check(false, std::string(nm) + " is not 8-byte aligned");
 }
 inline bool check_ptr4(const void* p, const char* nm) {
-  return check(p != nullptr, std::string(nm) + " is null") &&
-         check(aligned(p, 4), std::string(nm) + " is not 4-byte aligned");
+  if (p == nullptr) return check(false, std::string(nm) + " is null");
+  return aligned(p, 4) || check(false, std::string(nm) + " is not 4-byte aligned");
 }
 
 // Launch on `st`, with the programmatic-stream-serialization attribute when

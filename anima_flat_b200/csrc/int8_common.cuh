@@ -125,6 +125,11 @@ __device__ __forceinline__ f2_t code_pair(uint32_t w, int j) {
 cudaError_t quantize_rows(const void* x, const void* cols, int8_t* q, float* s, int64_t rows, int64_t K, int dtype,
                           cudaStream_t st);
 
+// The length of a row of codes.  (The message is made only where it is needed.)
+inline bool check_k(int64_t K, int64_t most) {
+  return (K >= 16 && K % 16 == 0 && K <= most) ||
+         check(false, "K must be a multiple of 16 in [16, " + std::to_string(most) + "], got " + std::to_string(K));
+}
 inline bool check_dtype(int dtype) { return check(dtype == kBf16 || dtype == kFp16, "dtype must be 0 (bf16) or 1 (fp16)"); }
 
 }  // namespace afb

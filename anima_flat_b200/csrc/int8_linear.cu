@@ -629,8 +629,7 @@ static bool check_linear(const void* w, const void* v, const void* bias, void* y
   return check(M >= 0 && M <= (1 << 30), "M must be in [0, 2^30]") &&
          check(N >= 1 && N <= (1 << 30), "N must be in [1, 2^30]") &&
          check(((M + 15) / 16) * ((N + kTileN - 1) / kTileN) <= (1 << 27), "M * N is too large") &&
-         check(K >= 16 && K % 16 == 0 && K <= most_k,
-               "K must be a multiple of 16 in [16, " + std::to_string(most_k) + "], got " + std::to_string(K)) &&
+         check_k(K, most_k) &&
          check_dtype(dtype) &&
          (M == 0 || (check_ptrs({w, y}, {"w", "y"}) && check(aligned(v, 4), "v is not 4-byte aligned") &&
                      check(aligned(bias, 2), "bias is not 2-byte aligned")));

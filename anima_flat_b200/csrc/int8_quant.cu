@@ -312,10 +312,7 @@ static cudaError_t launch_restore(const RestoreArgs& a, int dtype, cudaStream_t 
 
 // rows * K / 16 chunks of 256-thread blocks must fit the grid's x extent.
 static bool check_quant(int64_t rows, int64_t K, int dtype) {
-  int group = 0, cpl = 0;
-  return check(rows >= 0 && rows <= INT64_C(0x7fffffff), "rows must be in [0, 2^31)") &&
-         check(quant_shape<kPlain>(K, &group, &cpl),
-               "K must be a multiple of 16 in [16, 16384], got " + std::to_string(K)) &&
+  return check(rows >= 0 && rows <= INT64_C(0x7fffffff), "rows must be in [0, 2^31)") && check_k(K, 16384) &&
          check_dtype(dtype);
 }
 

@@ -593,7 +593,7 @@ extern "C" int afb_int8_wgrad(const void* dy, const void* q, const void* s, void
   ApiGuard g("afb_int8_wgrad");
   if (!check(rows >= 0 && rows <= (1 << 30), "rows must be in [0, 2^30]") ||
       !check(N >= 1 && N <= (1 << 20), "N must be in [1, 2^20]") ||
-      !check(K >= 16 && K % 16 == 0 && K <= (1 << 20), "K must be a multiple of 16 in [16, 2^20], got " + std::to_string(K)) ||
+      !check_k(K, 1 << 20) ||
       !check_dtype(dtype) || !check_ptrs({dw}, {"dw"}))
     return g.fail();
   cudaStream_t st = static_cast<cudaStream_t>(stream);

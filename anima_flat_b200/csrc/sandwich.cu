@@ -746,12 +746,12 @@ static bool check_sandwich(int64_t B, int64_t S, int64_t D, int dtype) {
   return check(B >= 0 && B <= 65535, "batch must be in [0, 65535]") &&
          check(S >= 0 && S <= (1 << 30), "seq must be in [0, 2^30]") &&
          check(B * S <= INT64_C(0x7fffffff), "batch * seq must be below 2^31") &&
-         check(D >= 8 && D % 8 == 0 && D <= kMaxRowDim,
-               "dim must be a multiple of 8 in [8, " + std::to_string(kMaxRowDim) + "], got " + std::to_string(D)) &&
+         ((D >= 8 && D % 8 == 0 && D <= kMaxRowDim) ||
+          check(false, "dim must be a multiple of 8 in [8, " + std::to_string(kMaxRowDim) + "], got " + std::to_string(D))) &&
          check_dtype(dtype);
 }
 static bool check_opt16(const void* p, const char* n) {
-  return check(aligned(p, 16), std::string(n) + " is not 16-byte aligned");
+  return aligned(p, 16) || check(false, std::string(n) + " is not 16-byte aligned");
 }
 
 cudaError_t read_status_sandwich(int* status, bool clear) { return tu_status(status, clear); }
