@@ -430,9 +430,8 @@ static cudaError_t launch_linear(const void* q, const void* w, LinearArgs a, int
                         split);
 }
 
-// Tokens of a tile and parts along k.  Up to 128 tokens one tile holds them
-// all; above, 256 (pairs of CTAs) where tiles of 128 x 256 still give every
-// multiprocessor one, else 128.  Few tiles are split along k, two blocks a
+// Tokens of a tile and parts along k, for single CTAs.  Up to 128 tokens one
+// tile holds them all; above, 128.  Few tiles are split along k, two blocks a
 // multiprocessor (264 fit in clusters of eight), into parts of four k blocks at
 // least, or two while half of the multiprocessors would have none: 512 x 8192 ->
 // 2048 14.8 us in 4 parts, 17.5 in 2; 128 x 2048 -> 2048 6.7 in 4, 8.2 in 8;
@@ -441,13 +440,29 @@ static void linear_shape(int M, int N, int K, int sms, int* bn, int* split) {
   const int64_t nt = (N + kTileN - 1) / kTileN;
   auto tiles = [&](int b) { return nt * ((M + b - 1) / b); };
   int b = 16;
-  while (b < 256 && b < M && (b < 128 || tiles(2 * b) >= sms)) b *= 2;
+  while (b < 128 && b < M) b *= 2;
   const int blocks = (K + kKBlock - 1) / kKBlock;
   int s = 1;
-  while (s < 8 && b < 256 && tiles(b) * s * 2 <= 2 * sms - 32 && blocks / (2 * s) >= (tiles(b) * s * 2 <= sms / 2 ? 2 : 4))
-    s *= 2;
+  while (s < 8 && tiles(b) * s * 2 <= 2 * sms - 32 && blocks / (2 * s) >= (tiles(b) * s * 2 <= sms / 2 ? 2 : 4)) s *= 2;
   *bn = b;
   *split = s;
+}
+
+// Whether pairs of CTAs take a product of more than 128 tokens.  Always where
+// 128 x 256 tiles would give every multiprocessor one.  For fewer, from eight
+// k blocks on, where they take less by what was measured: a pair 4 us and 0.21 a
+// k block and round of tiles; single CTAs 4 us, 7 in a cluster, and 0.30 a k
+// block of a part, 0.48 where two share a multiprocessor.  1024 x 2048 -> 2048
+// 8.2 us (11.2 single), 512 x 8192 -> 2048 17.1 (14.8).
+static bool linear_by_pairs(int M, int N, int K, int bn, int split, int sms) {
+  if (M <= 128) return false;
+  const int64_t nt = (N + kTileN - 1) / kTileN, blocks = (K + kKBlock - 1) / kKBlock;
+  if (nt * ((M + 255) / 256) >= sms) return true;
+  if (blocks < 8) return false;
+  const int64_t rounds = ((nt + 1) / 2 * ((M + 255) / 256) + sms / 2 - 1) / (sms / 2);
+  const int64_t ctas = nt * ((M + bn - 1) / bn) * split;
+  const int64_t single = (split > 1 ? 700 : 400) + (ctas + 2 * sms - 1) / (2 * sms) * (blocks / split) * (ctas > sms ? 48 : 30);
+  return 400 + rounds * blocks * 21 < single;
 }
 
 // Tokens of a pair's tile: of 256, 224, 192 and 160 the one whose whole rounds
@@ -476,7 +491,8 @@ static cudaError_t linear(const void* q, const void* w, const LinearArgs& a, cud
   if (d.error != cudaSuccess) return d.error;
   int bn, split;
   linear_shape(a.M, a.N, a.K, d.sms, &bn, &split);
-  if (bn == 256) return launch_pair<DT>(q, w, a, pair_tokens(a.M, a.N, d.sms / 2), st);
+  if (linear_by_pairs(a.M, a.N, a.K, bn, split, d.sms))
+    return launch_pair<DT>(q, w, a, pair_tokens(a.M, a.N, d.sms / 2), st);
   switch (bn) {
     case 16: return launch_linear<16, DT>(q, w, a, split, st);
     case 32: return launch_linear<32, DT>(q, w, a, split, st);

@@ -518,24 +518,35 @@ static cudaError_t launch_wgrad_pair(const void* dy, const void* q, WgradArgs a,
   return launch_cluster(int8_wgrad_pair_kernel<DT>, dim3(grid), dim3(kPairThreads), kPairSmem, 2, st, qmap, gmap, a, tiles);
 }
 
-// Columns of a tile and parts along the tokens: the narrowest tile that holds
-// all columns, up to 128, or 256 (pairs of CTAs) where that still gives every
-// multiprocessor a tile of 128 x 256.  Few tiles are split into parts of at
+// Columns of a tile and parts along the tokens, for single CTAs: the narrowest
+// tile that holds all columns, up to 128.  Few tiles are split into parts of at
 // least two stages: up to 64 columns two blocks share a multiprocessor and 264
 // run at once in clusters of eight; above, 132 in clusters of four but only 120
 // in clusters of eight (128 columns of 2048 channels: 12.2 us in 4 parts, 19.7
 // in 8).
 static void wgrad_shape(int T, int N, int K, int sms, int* bn, int* split) {
   const int64_t kt = (K + kCh - 1) / kCh;
-  auto tiles = [&](int b) { return kt * ((N + b - 1) / b); };
   int b = 16;
-  while (b < 256 && b < N && (b < 128 || tiles(2 * b) >= sms)) b *= 2;
+  while (b < 128 && b < N) b *= 2;
+  const int64_t tiles = kt * ((N + b - 1) / b);
   const int blocks = (T + kTok - 1) / kTok;
-  int s = 1;
   const int most = b <= 64 ? 8 : 4, fit = b <= 64 ? 2 * sms - 32 : sms - 16;
-  while (s < most && b < 256 && tiles(b) * s * 2 <= fit && blocks / (2 * s) >= 2) s *= 2;
+  int s = 1;
+  while (s < most && tiles * s * 2 <= fit && blocks / (2 * s) >= 2) s *= 2;
   *bn = b;
   *split = s;
+}
+
+// Whether pairs of CTAs take a gradient of more than 128 columns, by what was
+// measured: a pair 4 us and 0.34 a stage and round of tiles, single CTAs 5 us
+// and 0.37 a stage of a part and round.  4096 tokens: 2048 x 2048 29 us (55
+// single), 1024 x 1024 25 (18).
+static bool wgrad_by_pairs(int T, int N, int K, int split, int sms) {
+  if (N <= 128) return false;
+  const int64_t blocks = (T + kTok - 1) / kTok, kt = (K + kCh - 1) / kCh;
+  const int64_t pair_rounds = ((kt + 1) / 2 * ((N + 255) / 256) + sms / 2 - 1) / (sms / 2);
+  const int64_t rounds = (kt * ((N + 127) / 128) * split + sms - 1) / sms;
+  return 400 + pair_rounds * blocks * 34 < 500 + rounds * (blocks / split) * 37;
 }
 
 template <int DT>
@@ -544,7 +555,7 @@ static cudaError_t wgrad(const void* dy, const void* q, const WgradArgs& a, cuda
   if (d.error != cudaSuccess) return d.error;
   int bn, split;
   wgrad_shape(a.T, a.N, a.K, d.sms, &bn, &split);
-  if (bn == 256) return launch_wgrad_pair<DT>(dy, q, a, st);
+  if (wgrad_by_pairs(a.T, a.N, a.K, split, d.sms)) return launch_wgrad_pair<DT>(dy, q, a, st);
   switch (bn) {
     case 16: return launch_wgrad<16, DT>(dy, q, a, split, st);
     case 32: return launch_wgrad<32, DT>(dy, q, a, split, st);
