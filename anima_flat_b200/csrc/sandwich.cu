@@ -429,6 +429,13 @@ struct SandwichBwdArgs {
 // sums stay in its registers, so a row is read once.  Bulk copies keep the next
 // two pairs of every team on their way in shared memory: with the loads in the
 // row loop itself the kernel ran at 39% of memory speed, on their latency.
+//
+// All six sums of a row are taken at once, with t = x gate post, since
+//   sum m xh = r1 (sum gz t + r2 (sum p t - r2 mean(p zh) sum z t)):
+// one barrier a pair of rows, and dx in the pass that forms dz (8192 x 2048: 44.9
+// us, 46.0 with a barrier of its own for sum m xh).  With the sums' kernel below
+// 43.5 us, 4096 x 2048 27.8: memory speed, and 12 us that do not depend on the
+// rows (launches, first and last copies, the columns' sums).
 constexpr int kBwdRows = 2;    // rows a team holds at once
 constexpr int kBwdStages = 3;  // of kBwdRows rows each
 static size_t bwd_smem(int D) { return static_cast<size_t>(teams_of(D)) * kBwdStages * kBwdRows * 4 * D * 2; }
@@ -454,15 +461,7 @@ __device__ __forceinline__ float warp_sum8(const float (&v)[8]) {
   c += __shfl_xor_sync(kFull, c, 2);
   return c + __shfl_xor_sync(kFull, c, 1);
 }
-// Sums of two values: lane l returns that of value l / 16.
-__device__ __forceinline__ float warp_sum2(float v0, float v1) {
-  const bool up = threadIdx.x & 16;
-  float c = (up ? v1 : v0) + __shfl_xor_sync(kFull, up ? v0 : v1, 16);
-#pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) c += __shfl_xor_sync(kFull, c, o);
-  return c;
-}
-// The team's sum of value l / 4 or l / 16, for every lane l, from its warps' in
+// The team's sum of value l / 4, for every lane l, from its warps' in
 // red[value][warp] (zero above the team's warps).
 __device__ __forceinline__ float team_sum8(const float (*red)[16]) {
   const int lane = threadIdx.x & 31;
@@ -471,21 +470,14 @@ __device__ __forceinline__ float team_sum8(const float (*red)[16]) {
   c += __shfl_xor_sync(kFull, c, 2);
   return c + __shfl_xor_sync(kFull, c, 1);
 }
-__device__ __forceinline__ float team_sum2(const float (*red)[16]) {
-  const int lane = threadIdx.x & 31;
-  float c = red[lane >> 4][lane & 15];
-#pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) c += __shfl_xor_sync(kFull, c, o);
-  return c;
-}
-
 template <int DT>
 __global__ void __launch_bounds__(kTeamThreads, 1) sandwich_bwd_kernel(const SandwichBwdArgs a, int team_threads, int teams) {
   constexpr int R = kBwdRows, NS = kBwdStages;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[8 * NS];
-  // per team: sums of z^2, p z, x^2 of the rows by warp, and of m xh
-  __shared__ __align__(16) float red1[8][8][16], red2[8][R][16];
+  // per team, for steps in turn: the rows' sums by warp, of z^2, x^2, p z and
+  // gz t, and of p t and z t, with t = x gate post
+  __shared__ __align__(16) float red8[2][8][8][16], red4[2][8][4][16];
   const int lane = threadIdx.x & 31;
   const int team = static_cast<int>(threadIdx.x) / team_threads, tid = static_cast<int>(threadIdx.x) % team_threads;
   const int warp = tid >> 5;
@@ -500,9 +492,9 @@ __global__ void __launch_bounds__(kTeamThreads, 1) sandwich_bwd_kernel(const San
     for (int i = 0; i < NS; ++i) mbar_init(bar0 + 8 * i, 1);
     fence_mbar_init();
   }
-  for (int i = static_cast<int>(threadIdx.x); i < 8 * 8 * 16; i += static_cast<int>(blockDim.x)) {
-    (&red1[0][0][0])[i] = 0.0f;
-    if (i < 8 * R * 16) (&red2[0][0][0])[i] = 0.0f;
+  for (int i = static_cast<int>(threadIdx.x); i < 2 * 8 * 8 * 16; i += static_cast<int>(blockDim.x)) {
+    (&red8[0][0][0][0])[i] = 0.0f;
+    if (i < 2 * 8 * 4 * 16) (&red4[0][0][0][0])[i] = 0.0f;
   }
   __syncthreads();
   pdl_wait();
@@ -556,77 +548,74 @@ __global__ void __launch_bounds__(kTeamThreads, 1) sandwich_bwd_kernel(const San
         for (int t = 0; t < 4; ++t) st16(piece(k, t), make_uint4(0, 0, 0, 0));  // no such row
       }
     }
-    float sums[8] = {};
+    float sums[8] = {}, more[4] = {};
     if (col) {
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        f2_t g[4], z[4], x[4], s0 = 0, s1 = 0, s2 = 0;
+        f2_t g[4], z[4], x[4], gz[4] = {}, s0 = 0, s1 = 0, s2 = 0, s3 = 0, s4 = 0, s5 = 0;
         unpack4p<DT>(lds16(piece(k, 0)), g);
+        if (a.gz != nullptr) unpack4p<DT>(lds16(piece(k, 1)), gz);
         unpack4p<DT>(lds16(piece(k, 2)), z);
         unpack4p<DT>(lds16(piece(k, 3)), x);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          const f2_t p = mul2(g[j], pw[j]), t = mul2(x[j], gw[j]);
           s0 = fma2(z[j], z[j], s0);
-          s1 = fma2(mul2(g[j], pw[j]), z[j], s1);
-          s2 = fma2(x[j], x[j], s2);
+          s1 = fma2(x[j], x[j], s1);
+          s2 = fma2(p, z[j], s2);
+          s3 = fma2(gz[j], t, s3);
+          s4 = fma2(p, t, s4);
+          s5 = fma2(z[j], t, s5);
         }
         sums[k] = sum2(s0);
-        sums[2 + k] = sum2(s2);
-        sums[4 + k] = sum2(s1);
+        sums[2 + k] = sum2(s1);
+        sums[4 + k] = sum2(s2);
+        sums[6 + k] = sum2(s3);
+        more[k] = sum2(s4);
+        more[2 + k] = sum2(s5);
       }
     }
-    const float own = warp_sum8(sums);
-    if ((lane & 3) == 0) red1[team][lane >> 2][warp] = own;
+    const float own = warp_sum8(sums), own4 = warp_sum4(more);
+    if ((lane & 3) == 0) red8[i & 1][team][lane >> 2][warp] = own;
+    if ((lane & 7) == 0) red4[i & 1][team][lane >> 3][warp] = own4;
     named_bar_sync(1 + team, team_threads);
     // The team is done with pair i - 1: its stage takes pair i + 2.
     if (tid == 0 && ok && asked < mine) {
       fence_proxy_async_smem();
       request(asked++);
     }
-    // Lanes of the first four values turn them into reciprocal roots; the
-    // last two become the means of p zh.
-    const float all = team_sum8(red1[team]);
+    // Lanes of the first four values turn them into reciprocal roots.
+    const float all = team_sum8(red8[i & 1][team]), all4 = team_sum4(red4[i & 1][team]);
     const float root = rms_scale(all, inv_d, a.eps);
-    f2_t dm[R][4];  // dz gate post
-    float rx[R], part[R];
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-      const float rz = __shfl_sync(kFull, root, 4 * k);
-      rx[k] = __shfl_sync(kFull, root, 8 + 4 * k);
+      const float rz = __shfl_sync(kFull, root, 4 * k), rx = __shfl_sync(kFull, root, 8 + 4 * k);
       const float c = __shfl_sync(kFull, all, 16 + 4 * k) * rz * inv_d;  // mean(p zh)
-      f2_t g[4], z[4], x[4], gz[4] = {}, o[4], s3 = 0;
+      const float gzt = __shfl_sync(kFull, all, 24 + 4 * k);
+      const float pt = __shfl_sync(kFull, all4, 8 * k), zt = __shfl_sync(kFull, all4, 16 + 8 * k);
+      // mean(m xh)
+      const float d = __fmaf_rn(rz, __fmaf_rn(-c * rz, zt, pt), gzt) * rx * inv_d;
+      if (!col) continue;
+      f2_t g[4], z[4], x[4], gz[4] = {}, o[4];
       unpack4p<DT>(lds16(piece(k, 0)), g);
       if (a.gz != nullptr) unpack4p<DT>(lds16(piece(k, 1)), gz);
       unpack4p<DT>(lds16(piece(k, 2)), z);
       unpack4p<DT>(lds16(piece(k, 3)), x);
-      const f2_t rz2 = splat2(rz), rx2 = splat2(rx[k]), nc = splat2(-c);
+      const f2_t rz2 = splat2(rz), rx2 = splat2(rx), nc = splat2(-c), nd = splat2(-d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const f2_t zh = mul2(z[j], rz2), xh = mul2(x[j], rx2);
         const f2_t dz = fma2(rz2, fma2(zh, nc, mul2(g[j], pw[j])), gz[j]);
-        dm[k][j] = mul2(dz, gw[j]);
-        s3 = fma2(dm[k][j], xh, s3);
         P[j] = fma2(g[j], zh, P[j]);
         Q[j] = fma2(dz, xh, Q[j]);
         G[j] = add2(G[j], g[j]);
         o[j] = mul2(alpha, dz);
+        x[j] = mul2(rx2, fma2(xh, nd, mul2(dz, gw[j])));
       }
-      part[k] = col ? sum2(s3) : 0.0f;
-      if (col && r + k < rows) st16(a.dres + (b * a.S + r0 + r + k) * a.D + e, pack4p<DT>(o));
-    }
-    const float own2 = warp_sum2(part[0], part[1]);
-    if ((lane & 15) == 0) red2[team][lane >> 4][warp] = own2;
-    named_bar_sync(1 + team, team_threads);
-    const float mean = team_sum2(red2[team]) * inv_d;
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const f2_t nc = splat2(-__shfl_sync(kFull, mean, 16 * k)), rx2 = splat2(rx[k]);
-      if (col && r + k < rows) {
-        f2_t x[4];
-        unpack4p<DT>(lds16(piece(k, 3)), x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = mul2(rx2, fma2(mul2(x[j], rx2), nc, dm[k][j]));
-        st16(a.dx + (b * a.S + r0 + r + k) * a.D + e, pack4p<DT>(x));
+      if (r + k < rows) {
+        const int64_t to = (b * a.S + r0 + r + k) * a.D + e;
+        st16(a.dres + to, pack4p<DT>(o));
+        st16(a.dx + to, pack4p<DT>(x));
       }
     }
   }
@@ -662,6 +651,9 @@ __global__ void __launch_bounds__(kTeamThreads, 1) sandwich_bwd_kernel(const San
   }
 }
 
+constexpr int kFinCols = 16, kFinSlots = 16, kFinThreads = kFinCols * kFinSlots;
+constexpr int kFinBatch = 5;  // chunks that a thread has under way
+
 struct SandwichFinalArgs {
   const float* part;
   const uint16_t *gate, *scale;  // [B, D] or null
@@ -672,69 +664,65 @@ struct SandwichFinalArgs {
   int chunks, D;
 };
 
-// 32 columns a block.  Its 32 warps form 1, 2 or 4 groups, which take the
-// samples in turn; a group's warps sum its chunks, lane by column, then every
-// warp adds its group's sums of some columns.  Five chunks are asked for at once
-// (148 blocks' by 32 warps): the kernel is one round trip to L2 long.
+// 16 columns a block, so that 2048 columns take most multiprocessors; a thread
+// sums every 16th chunk (of a group's samples) of one column, then one thread a
+// sum and column adds the slots.  Five chunks are asked for at once: 148 blocks'
+// are two round trips to L2.  With 32 columns and 1024 threads, added by warps,
+// both kernels took 9.4 us for 64 x 2048, 8.1 so.
 template <int DT>
-__global__ void __launch_bounds__(1024) sandwich_final_kernel(const SandwichFinalArgs a) {
-  __shared__ float red[3][32][33];
-  __shared__ float both[2][4][33];  // dpre and dpost of the groups
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int groups = a.B >= 4 ? 4 : a.B >= 2 ? 2 : 1, per = 32 / groups;
-  const int g = warp / per, w = warp % per;
-  const int col0 = blockIdx.x * 32, cl = col0 + lane;
+__global__ void __launch_bounds__(kFinThreads) sandwich_final_kernel(const SandwichFinalArgs a) {
+  __shared__ float red[3][kFinSlots][kFinCols + 1];
+  __shared__ float both[4][2][kFinCols];  // dpre and dpost of the groups
+  const int t = static_cast<int>(threadIdx.x), c = t % kFinCols, at = static_cast<int>(blockIdx.x) * kFinCols + c;
+  const bool col = at < a.D;
+  // Groups of slots take samples in turn; a slot adds every `per`-th chunk.
+  const int groups = a.B >= 4 ? 4 : a.B >= 2 ? 2 : 1, per = kFinSlots / groups;
+  const int slot = t / kFinCols, g = slot / per, w = slot % per;
+  // The thread that adds the slots of sum i: 0 P, 1 Q, 2 gh.
+  const int sg = slot / 3, i = slot % 3;
+  uint16_t* out = i == 0 ? a.dscale : i == 1 ? a.dgate : a.dshift;
+  const uint16_t* factor = i == 0 ? a.scale : a.gate;
   pdl_wait();
   pdl_trigger();
-  float dsum[2][4] = {};  // of the columns w, w + per, ... : dpre, dpost (lane 0)
+  const float norm = !col || i == 2 ? 1.0f : __ldg((i == 0 ? a.pre : a.post) + at);
+  float dnorm = 0.0f;
   for (int64_t b0 = 0; b0 < a.B; b0 += groups) {
-    const int64_t b = b0 + g;
     float s[3] = {};
-    if (cl < a.D && b < a.B) {
-      const float* base = a.part + b * a.chunks * 3 * a.D + cl;
-      for (int n0 = w; n0 < a.chunks; n0 += 5 * per) {
-        float v[5][3];
+    if (col && b0 + g < a.B) {
+      const float* base = a.part + (b0 + g) * a.chunks * 3 * a.D + at;
+      for (int n0 = w; n0 < a.chunks; n0 += kFinBatch * per) {
+        float v[kFinBatch][3];
 #pragma unroll
-        for (int u = 0; u < 5; ++u)
+        for (int u = 0; u < kFinBatch; ++u)
 #pragma unroll
-          for (int i = 0; i < 3; ++i) {
+          for (int k = 0; k < 3; ++k) {
             const int n = n0 + u * per;
-            v[u][i] = n < a.chunks ? __ldcg(base + (static_cast<int64_t>(n) * 3 + i) * a.D) : 0.0f;
+            v[u][k] = n < a.chunks ? __ldcg(base + (static_cast<int64_t>(n) * 3 + k) * a.D) : 0.0f;
           }
 #pragma unroll
-        for (int u = 0; u < 5; ++u)
+        for (int u = 0; u < kFinBatch; ++u)
 #pragma unroll
-          for (int i = 0; i < 3; ++i) s[i] += v[u][i];
+          for (int k = 0; k < 3; ++k) s[k] += v[u][k];
       }
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) red[i][warp][lane] = s[i];
+    for (int k = 0; k < 3; ++k) red[k][slot][c] = s[k];
     __syncthreads();
-    for (int k = 0; w + k * per < 32; ++k) {
-      const int c = w + k * per, at = col0 + c;
-#pragma unroll
-      for (int i = 0; i < 3; ++i) s[i] = warp_sum(lane < per ? red[i][g * per + lane][c] : 0.0f);
-      if (lane == 0 && at < a.D && b < a.B) {
-        const int64_t o = b * a.D + at;
-        dsum[0][k] = __fmaf_rn(a.scale ? load1<DT>(a.scale + o) : 1.0f, s[0], dsum[0][k]);
-        dsum[1][k] = __fmaf_rn(a.gate ? load1<DT>(a.gate + o) : 1.0f, s[1], dsum[1][k]);
-        if (a.dscale) a.dscale[o] = static_cast<uint16_t>(pack2<DT>(__ldg(a.pre + at) * s[0], 0.0f));
-        if (a.dgate) a.dgate[o] = static_cast<uint16_t>(pack2<DT>(__ldg(a.post + at) * s[1], 0.0f));
-        if (a.dshift) a.dshift[o] = static_cast<uint16_t>(pack2<DT>(s[2], 0.0f));
-      }
+    if (col && sg < groups && b0 + sg < a.B) {
+      const int64_t o = (b0 + sg) * a.D + at;
+      float sum = 0.0f;
+      for (int k = 0; k < per; ++k) sum += red[i][sg * per + k][c];
+      if (i < 2) dnorm = __fmaf_rn(factor ? load1<DT>(factor + o) : 1.0f, sum, dnorm);
+      if (out) out[o] = static_cast<uint16_t>(pack2<DT>(norm * sum, 0.0f));
     }
     __syncthreads();
   }
-  if (lane == 0)
-    for (int k = 0; w + k * per < 32; ++k) {
-      both[0][g][w + k * per] = dsum[0][k];
-      both[1][g][w + k * per] = dsum[1][k];
-    }
+  if (sg < groups && i < 2) both[sg][i][c] = dnorm;
   __syncthreads();
-  if (warp < 2 && cl < a.D) {
+  if (slot < 2 && col) {
     float sum = 0.0f;
-    for (int i = 0; i < groups; ++i) sum += both[warp][i][lane];
-    (warp == 0 ? a.dpre : a.dpost)[cl] = sum;
+    for (int k = 0; k < groups; ++k) sum += both[k][slot][c];
+    (slot == 0 ? a.dpre : a.dpost)[at] = sum;
   }
 }
 
@@ -870,7 +858,7 @@ extern "C" int afb_sandwich_norm_bwd(const void* gh, const void* gz, const void*
   e = dtype == kBf16 ? launch_pdl(sandwich_bwd_kernel<kBf16>, grid, block, smem, st, a, team, teams)
                      : launch_pdl(sandwich_bwd_kernel<kFp16>, grid, block, smem, st, a, team, teams);
   if (e != cudaSuccess) return g.done(e);
-  const dim3 fg(static_cast<unsigned>((dim + 31) / 32));
-  return g.done(dtype == kBf16 ? launch_pdl(sandwich_final_kernel<kBf16>, fg, dim3(1024), 0, st, f)
-                               : launch_pdl(sandwich_final_kernel<kFp16>, fg, dim3(1024), 0, st, f));
+  const dim3 fg(static_cast<unsigned>((dim + kFinCols - 1) / kFinCols));
+  return g.done(dtype == kBf16 ? launch_pdl(sandwich_final_kernel<kBf16>, fg, dim3(kFinThreads), 0, st, f)
+                               : launch_pdl(sandwich_final_kernel<kFp16>, fg, dim3(kFinThreads), 0, st, f));
 }
