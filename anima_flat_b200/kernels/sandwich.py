@@ -15,7 +15,7 @@ from __future__ import annotations
 
 import torch
 
-from .._lib import workspace
+from .._lib import load
 from .common import HALF_TYPES, _check_half, _check_same_device, _check_vec, _dense, _launch, _plain
 
 __all__ = ["sandwich_norm", "sandwich_norm_bwd", "sandwich_norm_int8"]
@@ -54,13 +54,17 @@ def _fwd_int8(x, residual, gate, post_weight, pre_weight, shift, scale, residual
 def _bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale, residual_scale, eps):
     B, S, D = z.shape
     dx, dres = torch.empty_like(x), torch.empty_like(z)
-    dgate, dshift, dscale = (z.new_empty((B, D)) for _ in range(3))
+    vec = gate if gate is not None else scale
+    if vec is None:
+        vec = z.new_empty((B, D))
+    dgate, dshift, dscale = torch.empty_like(vec), torch.empty_like(vec), torch.empty_like(vec)
     dpost, dpre = torch.empty_like(post_weight), torch.empty_like(pre_weight)
     if z.numel() == 0:
         for t in (dgate, dshift, dscale, dpost, dpre):
             t.zero_()
         return dx, dres, dgate, dpost, dpre, dshift, dscale
-    ws, nbytes = workspace("afb_sandwich_norm_bwd", z.device, B, S, D)
+    nbytes = load().afb_sandwich_norm_bwd_workspace(B, S, D)
+    ws = z.new_empty(nbytes, dtype=torch.int8)
     _launch("afb_sandwich_norm_bwd", z, gh.data_ptr(), _ptr(gz), z.data_ptr(), x.data_ptr(), _ptr(gate),
             post_weight.data_ptr(), pre_weight.data_ptr(), _ptr(scale), dx.data_ptr(), dres.data_ptr(),
             dgate.data_ptr(), dpost.data_ptr(), dpre.data_ptr(), dshift.data_ptr(), dscale.data_ptr(),
