@@ -434,8 +434,10 @@ struct SandwichBwdArgs {
 //   sum m xh = r1 (sum gz t + r2 (sum p t - r2 mean(p zh) sum z t)):
 // one barrier a pair of rows, and dx in the pass that forms dz (8192 x 2048: 44.9
 // us, 46.0 with a barrier of its own for sum m xh).  With the sums' kernel below
-// 43.5 us, 4096 x 2048 27.8: memory speed, and 12 us that do not depend on the
-// rows (launches, first and last copies, the columns' sums).
+// 43.5 us, 4096 x 2048 27.8, some 12 of which do not depend on the rows (launches,
+// first and last copies, the columns' sums).  In the row loop 16 warps fill 52%
+// of the issue slots, with 43 instructions an element; they wait for barriers and
+// shared memory in equal parts.
 constexpr int kBwdRows = 2;    // rows a team holds at once
 constexpr int kBwdStages = 3;  // of kBwdRows rows each
 static size_t bwd_smem(int D) { return static_cast<size_t>(teams_of(D)) * kBwdStages * kBwdRows * 4 * D * 2; }
