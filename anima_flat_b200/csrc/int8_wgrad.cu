@@ -3,10 +3,14 @@
 // over the tokens t, with the codes and scales that the forward product read.
 //
 // The sum runs along the rows of both operands, so both enter the matrix
-// instruction with their k index (the token) outermost: dy as it lies, by TMA;
-// the codes after groups of four warps have turned a stage's 64 tokens x 128 channels
-// into 16-bit floats, each value q s rounded once (the codes times a scale of
-// their own token fit no exponent of the instruction).  The sum is fp32.
+// instruction with their k index (the token) outermost, after groups of four
+// warps have turned a stage of 64 tokens into its operands.  A token's scale
+// goes with dy: the codes are exact in bf16, and g = dy s, formed in fp32, enters
+// as the two bf16 values hi = RN(g) and lo = RN(g - hi), whose sum is g to 2^-16
+// of it (2^-8 of bf16's half-step, 2^-5 of fp16's).  Both products add into one
+// fp32 sum.  With q s rounded to 16 bits instead, one product is enough, but the
+// error is 1.4 times that of rounding dw once, and fp16 ends at 65504 where codes
+// with fp32 scales do not; bf16 has fp32's range.
 //
 // A tile is 128 channels (tensor-memory lanes) by BN columns of dy.  For an
 // adapter's few columns the kernel reads the codes once at memory speed; for a
@@ -32,13 +36,15 @@ constexpr int kTok = 64;  // tokens of a stage
 constexpr int kCh = 128;  // channels of a tile
 
 // A stage's copies (codes, and BN columns of dy in chunks of 64 at most) and
-// its converted operand have rings of their own, since copies take longest.
-// Two blocks share a multiprocessor up to 64 columns: with one, 120 blocks at
-// most run at once in clusters of eight.
+// its converted codes have rings of their own, since copies take longest.  hi
+// takes the place of dy, and lo that of the codes; what of it does not fit there
+// (a second chunk) follows the converted codes.  Two blocks share a
+// multiprocessor up to 64 columns: with one, 120 blocks at most run at once in
+// clusters of eight.
 __host__ __device__ constexpr int wg_width(int bn) { return bn < 64 ? bn : 64; }  // columns of a chunk
 __host__ __device__ constexpr int wg_chunks(int bn) { return bn / wg_width(bn); }
 __host__ __device__ constexpr int wg_raw_bytes(int bn) { return kTok * kCh + bn * kTok * 2; }
-__host__ __device__ constexpr int wg_conv_bytes() { return kCh * kTok * 2; }
+__host__ __device__ constexpr int wg_conv_bytes(int bn) { return kCh * kTok * 2 + (wg_chunks(bn) - 1) * kTok * 128; }
 __host__ __device__ constexpr int wg_raw(int bn) { return bn == 16 || bn >= 128 ? 6 : 3; }
 // Groups of four warps that convert, one for each converted stage, and then
 // write the results.  Sixteen warps on one stage after another took 0.58 us a
@@ -47,13 +53,11 @@ __host__ __device__ constexpr int wg_raw(int bn) { return bn == 16 || bn >= 128 
 // behind its barrier, not two.
 constexpr int kGroups = 3;
 constexpr int kWgThreads = 64 + 128 * kGroups;
-__host__ __device__ constexpr int wg_smem(int bn) { return kGroups * wg_conv_bytes() + wg_raw(bn) * wg_raw_bytes(bn) + 1024; }
+__host__ __device__ constexpr int wg_smem(int bn) { return kGroups * wg_conv_bytes(bn) + wg_raw(bn) * wg_raw_bytes(bn) + 1024; }
 __host__ __device__ constexpr int wg_tmem(int bn) { return bn < 32 ? 32 : bn; }
 
-// Sixteen codes to two 16-byte pieces of the 16-bit type, times the scale.
-template <int DT>
-__device__ __forceinline__ void convert16(const uint4 q, float s, uint4& lo, uint4& hi) {
-  const f2_t s2 = splat2(s);
+// Sixteen codes to two 16-byte pieces of bf16.
+__device__ __forceinline__ void convert16(const uint4 q, uint4& lo, uint4& hi) {
   uint32_t o[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -64,30 +68,65 @@ __device__ __forceinline__ void convert16(const uint4 q, float s, uint4& lo, uin
     const f2_t b = f2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)),
                       __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)));
     const f2_t base = splat2(8388736.0f);
-    o[2 * j] = pack2<DT>(mul2(sub2(a, base), s2));
-    o[2 * j + 1] = pack2<DT>(mul2(sub2(b, base), s2));
+    o[2 * j] = pack2<kBf16>(sub2(a, base));
+    o[2 * j + 1] = pack2<kBf16>(sub2(b, base));
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]);
   hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
+__device__ __forceinline__ void sts16a(uint32_t addr, const uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // A token's 16 channels 16 part .. of a stage, converted, to the operand at
 // `dst`: chunk of 64 channels, row of the token, 16-byte pieces swizzled by it.
-template <int DT>
-__device__ __forceinline__ void put_converted(uint32_t dst, int t, int part, const uint4 code, float s) {
+__device__ __forceinline__ void put_converted(uint32_t dst, int t, int part, const uint4 code) {
   uint4 lo, hi;
-  convert16<DT>(code, s, lo, hi);
+  convert16(code, lo, hi);
   const uint32_t row = dst + (part >> 2) * (kTok * 128) + t * 128;
   const uint32_t p0 = ((2 * (part & 3)) ^ (t & 7)) * 16;
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + p0), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (p0 ^ 16)), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+  sts16a(row + p0, lo);
+  sts16a(row + (p0 ^ 16), hi);
+}
+
+// The warp's 16 rows of a chunk of dy at `src`, ROW bytes a token, times their
+// scales: hi in their place, lo at `dst`.  A piece's place within the swizzled
+// rows stays what it is.  The scale of row r comes from lane half + r.  An
+// infinity or a NaN is in hi alone: as lo it would make a NaN of either.
+template <int DT, int ROW>
+__device__ __forceinline__ void split_rows(uint32_t src, uint32_t dst, float scales, int half) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < ROW / 32; ++j) {
+    const int p = lane + 32 * j;
+    const f2_t s = splat2(__shfl_sync(kFull, scales, half + p / (ROW / 16)));
+    const uint4 v = lds16a(src + 16 * p);
+    uint4 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f2_t g = mul2(unpack2<DT>(word(v, k)), s);
+      const uint32_t h = pack2<kBf16>(g);
+      const f2_t r = sub2(g, unpack2<kBf16>(h));
+      const float a = f2lo(r), b = f2hi(r);
+      word_ref(hi, k) = h;
+      word_ref(lo, k) = pack2<kBf16>(fabsf(a) < 0x1p127f ? a : 0.0f, fabsf(b) < 0x1p127f ? b : 0.0f);
+    }
+    sts16a(src + 16 * p, hi);
+    sts16a(dst + 16 * p, lo);
+  }
+}
+
+// Both operands bf16, outermost along k (bits 15, 16), `rows` by `cols`, fp32 sums.
+__host__ __device__ constexpr uint32_t wg_idesc(int rows, int cols) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (uint32_t(cols >> 3) << 17) | (uint32_t(rows >> 4) << 24);
 }
 
 template <int BN, int DT>
 __global__ void __launch_bounds__(kWgThreads, BN <= 64 ? 2 : 1)
 int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
                   const WgradArgs a, int split) {
-  constexpr int R = wg_raw(BN), RB = wg_raw_bytes(BN), CB = wg_conv_bytes(), G = kGroups;
+  constexpr int R = wg_raw(BN), RB = wg_raw_bytes(BN), CB = wg_conv_bytes(BN), G = kGroups;
   constexpr int kGOff = kTok * kCh, kRow = wg_width(BN) * 2;  // bytes of a chunk's row
   static_assert(R % G == 0, "");
   extern __shared__ uint8_t dyn[];
@@ -102,7 +141,7 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
     prefetch_map(&gmap);
     for (int i = 0; i < R; ++i) {
       mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, 5);  // the converting warps, and the matrix instructions
+      mbar_init(empty + 8 * i, 1);
     }
     for (int i = 0; i < G; ++i) {
       mbar_init(conv + 8 * i, 4);
@@ -150,21 +189,24 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
     if (!ok)  // copies still in flight land before the block ends
       for (int i = sent > R ? sent - R : 0; i < sent; ++i) mbar_wait(full + 8 * (i % R), (i / R) & 1);
   } else if (warp == 1) {
-    // fp32 sums; both operands 16-bit floats, outermost along k (bits 15, 16).
-    constexpr uint32_t type = DT == kBf16 ? 1u : 0u;
-    constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) |
-                               (uint32_t(BN >> 3) << 17) | (uint32_t(kCh >> 4) << 24);
+    constexpr uint32_t idesc = wg_idesc(kCh, BN), idesc_lo = wg_idesc(kCh, wg_width(BN));
     const uint64_t ca = smem_desc(ring, kTok * 128, 1024);
     const uint64_t cb = smem_desc(raw + kGOff, kTok * kRow, 8 * kRow, kRow);
+    const uint64_t cl = smem_desc(raw, kTok * kRow, 8 * kRow, kRow);
     for (int it = 0; it < nb; ++it) {
       const int st = it % R, cs = it % G;
-      if (!mbar_wait(full + 8 * st, (it / R) & 1) || !mbar_wait(conv + 8 * cs, (it / G) & 1)) break;
+      if (!mbar_wait(conv + 8 * cs, (it / G) & 1)) break;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t da = ca + static_cast<uint64_t>(cs * (CB >> 4)), db = cb + static_cast<uint64_t>(st * (RB >> 4));
+        const uint64_t dl = cl + static_cast<uint64_t>(st * (RB >> 4));
 #pragma unroll
-        for (int k = 0; k < kTok / 16; ++k)  // 16 tokens: two groups of 8 rows
+        for (int k = 0; k < kTok / 16; ++k) {  // 16 tokens: two groups of 8 rows
           mma_f16(tmem, da + k * (2048 >> 4), db + k * (16 * kRow >> 4), idesc, it > 0 || k > 0);
+          mma_f16(tmem, da + k * (2048 >> 4), dl + k * (2048 >> 4), idesc_lo, true);
+          if (wg_chunks(BN) > 1)  // after the converted codes
+            mma_f16(tmem + 64, da + k * (2048 >> 4), da + ((kCh * kTok * 2 + k * 2048) >> 4), idesc_lo, true);
+        }
         // the last ones are not waited for
         if (it + R < nb) mma_commit(empty + 8 * st);
         if (it + G < nb) mma_commit(cempty + 8 * cs);
@@ -175,13 +217,14 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
     __syncwarp();
   } else if (warp >= 2) {
     // A warp converts 16 tokens of a stage, four at a time: 8 lanes read a
-    // token's 128 codes.  Lane l keeps the scale of the warp's token l % 16, in
-    // this stage of the group or its next one (l / 16), and asks for the two
-    // after them when these begin, so that no stage waits for the load.
+    // token's 128 codes.  Its lo rows then take the place of its own codes, 2048
+    // bytes.  Lane l keeps the scale of the warp's token l % 16, in this stage of
+    // the group or its next one (l / 16), and asks for the two after them when
+    // these begin, so that no stage waits for the load.
     const int w = (warp - 2) & 3, part = lane & 7;
     auto scale_at = [&](int it) {
       const int at = it + (lane >> 4) * G;
-      const int t = (b0 + at) * kTok + ((lane >> 2) & 3) * 16 + w * 4 + (lane & 3);
+      const int t = (b0 + at) * kTok + w * 16 + (lane & 15);
       return at < nb && t < a.T ? __ldcg(a.s + t) : 0.0f;
     };
     const int g = (warp - 2) >> 2;
@@ -190,7 +233,7 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
     int half = 0;
     for (int it = g; it < nb; it += G, half ^= 16) {
       const int st = it % R;
-      const uint32_t src = raw + st * RB;
+      const uint32_t src = raw + st * RB + w * 2048, dy = raw + st * RB + kGOff + w * 16 * kRow;
       if (half == 0) {
         now = next;
         next = scale_at(it + 2 * G);
@@ -199,19 +242,15 @@ int8_wgrad_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
       if (it >= G && !mbar_wait(cempty + 8 * g, ((it / G) - 1) & 1)) break;
       uint4 code[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) code[i] = lds16a(src + (i * 16 + w * 4 + (lane >> 3)) * kCh + part * 16);
+      for (int i = 0; i < 4; ++i) code[i] = lds16a(src + (4 * i + (lane >> 3)) * kCh + part * 16);
+      __syncwarp();  // all of the warp's codes are read
+      split_rows<DT, kRow>(dy, src, now, half);
+      if (wg_chunks(BN) > 1) split_rows<DT, kRow>(dy + kTok * kRow, dst + kCh * kTok * 2 + w * 2048, now, half);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = i * 16 + w * 4 + (lane >> 3);
-        const float sc = __shfl_sync(kFull, now, half + i * 4 + (lane >> 3));
-        put_converted<DT>(dst, t, part, code[i], sc);
-      }
+      for (int i = 0; i < 4; ++i) put_converted(dst, w * 16 + 4 * i + (lane >> 3), part, code[i]);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(conv + 8 * g);
-        mbar_arrive(empty + 8 * st);
-      }
+      if (lane == 0) mbar_arrive(conv + 8 * g);
     }
     done = mbar_wait(accf, 0);
     tc_fence_after();
@@ -286,14 +325,15 @@ static cudaError_t launch_wgrad(const void* dy, const void* q, WgradArgs a, int 
 }
 
 // The same for many columns, by pairs of CTAs: a tile is 256 channels by 256
-// columns, a CTA converts and emits its 128 channels and brings half of the
-// columns; the first CTA issues the matrix instructions for both.  Codes, dy
-// and converted stages have rings of their own: a stage's copies take about
-// 1500 cycles and its conversion 700, its matrix instructions 512, so codes are
-// asked for eight stages ahead, dy five, and four are converted at a time.
+// columns, a CTA converts and emits its 128 channels and brings and converts half
+// of the columns; the first CTA issues the matrix instructions for both.  Codes,
+// dy (then hi) and converted stages (codes, then lo) have rings of their own.  A
+// stage's matrix instructions take 1024 cycles, and its bytes about 1280 of shared
+// memory's: 4096 tokens, 8192 x 2048 235 us, the matrix units at the measured
+// sustained rate 197.
 constexpr int kPairCols = 256;
-constexpr int kQRing = 8, kDRing = 5, kCRing = 4;
-constexpr int kQBytes = kTok * kCh, kDBytes = kPairCols / 2 * kTok * 2, kCBytes = kCh * kTok * 2;
+constexpr int kQRing = 3, kDRing = 6, kCRing = 3;
+constexpr int kQBytes = kTok * kCh, kDBytes = kPairCols / 2 * kTok * 2, kABytes = kCh * kTok * 2, kCBytes = kABytes + kDBytes;
 constexpr int kPairSmem = kQRing * kQBytes + kDRing * kDBytes + kCRing * kCBytes + 1024;
 // Copies of dy, matrix instructions, copies of codes, one idle; four warps of
 // the epilogue; kCRing groups of four that convert.
@@ -303,8 +343,8 @@ template <int DT>
 __global__ void __launch_bounds__(kPairThreads, 1)
 int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
                        const WgradArgs a, int tiles) {
-  // a group meets its stage of either ring in every phase
-  static_assert(kQRing % kCRing == 0, "");
+  // a group meets its stages of every ring in every phase
+  static_assert(kQRing % kCRing == 0 && kDRing % kCRing == 0, "");
   constexpr int kBars = 2 * (kQRing + kDRing + kCRing) + 4;
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[kBars];
@@ -356,7 +396,6 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
   auto column0 = [&](int tile) { return (tile / a.ktiles) * kPairCols; };
 
   if (warp == 0) {
-    const uint32_t dfull0 = peer_addr(dfull, 0);
     int it = 0, sent = 0;
     bool ok = true;
     for (int tile = first; ok && tile < tiles; tile += step) {
@@ -368,18 +407,16 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
           break;
         }
         if (elect_one()) {
-          if (rank == 0) mbar_arrive_expect_tx(dfull + 8 * st, 2 * kDBytes);
+          mbar_arrive_expect_tx(dfull + 8 * st, kDBytes);
 #pragma unroll
           for (int c = 0; c < kPairCols / 128; ++c)
-            tma_load_pair(dring + st * kDBytes + c * kTok * 128, &gmap, n0 + 64 * c, t * kTok, dfull0 + 8 * st);
+            tma_load(dring + st * kDBytes + c * kTok * 128, &gmap, n0 + 64 * c, t * kTok, dfull + 8 * st);
         }
         __syncwarp();
         sent = it + 1;
       }
     }
-    // After a wait that gave up: the first CTA's barriers count both CTAs'
-    // copies, and neither leaves before the cluster's last barrier.
-    if (!ok && rank == 0)
+    if (!ok)  // copies still in flight land before the block ends
       for (int i = sent > kDRing ? sent - kDRing : 0; i < sent; ++i) mbar_wait(dfull + 8 * (i % kDRing), (i / kDRing) & 1);
   } else if (warp == 2) {
     int it = 0, sent = 0;
@@ -404,9 +441,7 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
       for (int i = sent > kQRing ? sent - kQRing : 0; i < sent; ++i) mbar_wait(qfull + 8 * (i % kQRing), (i / kQRing) & 1);
   } else if (warp == 1) {
     if (rank == 0) {
-      constexpr uint32_t type = DT == kBf16 ? 1u : 0u;
-      constexpr uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) |
-                                 (uint32_t(kPairCols >> 3) << 17) | (uint32_t(2 * kCh >> 4) << 24);
+      constexpr uint32_t idesc = wg_idesc(2 * kCh, kPairCols);
       const uint64_t ca = smem_desc(cring, kTok * 128, 1024), cb = smem_desc(dring, kTok * 128, 1024);
       int it = 0;
       bool ok = true;
@@ -416,7 +451,7 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
         tc_fence_after();
         for (int t = 0; t < blocks; ++t, ++it) {
           const int ds = it % kDRing, cs = it % kCRing;
-          if (!mbar_wait_cluster(dfull + 8 * ds, (it / kDRing) & 1) || !mbar_wait_cluster(cfull + 8 * cs, (it / kCRing) & 1)) {
+          if (!mbar_wait_cluster(cfull + 8 * cs, (it / kCRing) & 1)) {
             ok = false;
             break;
           }
@@ -425,8 +460,10 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
             const uint64_t da = ca + static_cast<uint64_t>(cs * (kCBytes >> 4));
             const uint64_t db = cb + static_cast<uint64_t>(ds * (kDBytes >> 4));
 #pragma unroll
-            for (int k = 0; k < kTok / 16; ++k)
+            for (int k = 0; k < kTok / 16; ++k) {
               mma_f16_pair(tmem + buf * kPairCols, da + k * (2048 >> 4), db + k * (2048 >> 4), idesc, t > 0 || k > 0);
+              mma_f16_pair(tmem + buf * kPairCols, da + k * (2048 >> 4), da + ((kABytes + k * 2048) >> 4), idesc, true);
+            }
             // No arrival is under way to the other CTA when a CTA leaves:
             // only those that someone waits for are made.
             if (it + kDRing < mine * blocks) mma_commit_pair(dempty + 8 * ds);
@@ -445,29 +482,28 @@ int8_wgrad_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_co
     const uint32_t cfull0 = peer_addr(cfull, 0);
     auto scale_at = [&](int it) {
       const int at = it + (lane >> 4) * kCRing;
-      const int t = (at % blocks) * kTok + ((lane >> 2) & 3) * 16 + w * 4 + (lane & 3);
+      const int t = (at % blocks) * kTok + w * 16 + (lane & 15);
       return at < total && t < a.T ? __ldcg(a.s + t) : 0.0f;
     };
     float now = 0.0f, next = scale_at(g);
     int half = 0;
     for (int it = g; it < total; it += kCRing, half ^= 16) {
-      const int qs = it % kQRing;
-      const uint32_t dst = cring + g * kCBytes, src = qring + qs * kQBytes;
+      const int qs = it % kQRing, ds = it % kDRing;
+      const uint32_t dst = cring + g * kCBytes, src = qring + qs * kQBytes + w * 2048, dy = dring + ds * kDBytes + w * 2048;
       if (half == 0) {
         now = next;
         next = scale_at(it + 2 * kCRing);
       }
-      if (!mbar_wait(qfull + 8 * qs, (it / kQRing) & 1)) break;
+      if (!mbar_wait(qfull + 8 * qs, (it / kQRing) & 1) || !mbar_wait(dfull + 8 * ds, (it / kDRing) & 1)) break;
       if (it >= kCRing && !mbar_wait(cempty + 8 * g, ((it / kCRing) - 1) & 1)) break;
       uint4 code[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) code[i] = lds16a(src + (i * 16 + w * 4 + (lane >> 3)) * kCh + part * 16);
+      for (int i = 0; i < 4; ++i) code[i] = lds16a(src + (4 * i + (lane >> 3)) * kCh + part * 16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = i * 16 + w * 4 + (lane >> 3);
-        const float sc = __shfl_sync(kFull, now, half + i * 4 + (lane >> 3));
-        put_converted<DT>(dst, t, part, code[i], sc);
-      }
+      for (int c = 0; c < kPairCols / 128; ++c)
+        split_rows<DT, 128>(dy + c * kTok * 128, dst + kABytes + c * kTok * 128 + w * 2048, now, half);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) put_converted(dst, w * 16 + 4 * i + (lane >> 3), part, code[i]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -522,8 +558,7 @@ static cudaError_t launch_wgrad_pair(const void* dy, const void* q, WgradArgs a,
 // tile that holds all columns, up to 128.  Few tiles are split into parts of at
 // least two stages: up to 64 columns two blocks share a multiprocessor and 264
 // run at once in clusters of eight; above, 132 in clusters of four but only 120
-// in clusters of eight (128 columns of 2048 channels: 12.2 us in 4 parts, 19.7
-// in 8).
+// in clusters of eight (128 columns of 2048 channels: 18.1 us in 4 parts).
 static void wgrad_shape(int T, int N, int K, int sms, int* bn, int* split) {
   const int64_t kt = (K + kCh - 1) / kCh;
   int b = 16;
@@ -538,15 +573,15 @@ static void wgrad_shape(int T, int N, int K, int sms, int* bn, int* split) {
 }
 
 // Whether pairs of CTAs take a gradient of more than 128 columns, by what was
-// measured: a pair 4 us and 0.34 a stage and round of tiles, single CTAs 5 us
-// and 0.37 a stage of a part and round.  4096 tokens: 2048 x 2048 29 us (55
-// single), 1024 x 1024 25 (18).
+// measured: a pair 4 us and 0.75 a stage and round of tiles, single CTAs 5 us
+// and 0.72 a stage of a part and round.  4096 tokens: 2048 x 2048 57 us (101
+// single), 1024 x 1024 51 (30).
 static bool wgrad_by_pairs(int T, int N, int K, int split, int sms) {
   if (N <= 128) return false;
   const int64_t blocks = (T + kTok - 1) / kTok, kt = (K + kCh - 1) / kCh;
   const int64_t pair_rounds = ((kt + 1) / 2 * ((N + 255) / 256) + sms / 2 - 1) / (sms / 2);
   const int64_t rounds = (kt * ((N + 127) / 128) * split + sms - 1) / sms;
-  return 400 + pair_rounds * blocks * 34 < 500 + rounds * (blocks / split) * 37;
+  return 400 + pair_rounds * blocks * 75 < 500 + rounds * (blocks / split) * 72;
 }
 
 template <int DT>

@@ -468,7 +468,8 @@ def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tens
         s: Their scales, one per token.
 
     Returns:
-        ``[N, K]``, dtype of ``dy``, summed in fp32.
+        ``[N, K]``, dtype of ``dy``: an fp32 sum, rounded once.  The codes may stand for
+        values that this type does not hold (those of a bf16 row with an fp16 ``dy``).
 
     Raises:
         ValueError: On tensors off CUDA or unsupported dtypes or shapes.

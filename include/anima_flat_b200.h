@@ -310,7 +310,7 @@ int afb_int8_linear_x(const void* x, const void* cols, const void* w, const void
                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* dw[n, k] = sum_t dy[t, n] q[t, k] s[t], summed in fp32 in an order that the
- * sizes fix.  dy [rows, N]; q [rows, K], K a multiple of 16 up to 2^20;
+ * sizes fix; dy s is held to 2^-16 of it, in the range of fp32 for either type.  dy [rows, N]; q [rows, K], K a multiple of 16 up to 2^20;
  * s [rows]; dw [N, K] of `dtype` (zero where rows = 0).  Workspace as the query
  * says (none where N is a multiple of 8), 16-byte aligned, overwritten. */
 size_t afb_int8_wgrad_workspace(int64_t rows, int64_t N, int64_t K);

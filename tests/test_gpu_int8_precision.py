@@ -1,0 +1,88 @@
+"""Accuracy of the 8-bit operators where a value held in 16 bits on the way would show.
+
+u is the half-step of the 16-bit type, 2^-8 (bf16) or 2^-11 (fp16).
+
+int8_wgrad: dy s is formed in fp32 and held as two bf16 values, within 2^-16 of
+it, and two products a token go into an fp32 sum, whose additions may cut off
+2^-23 of it: u |dw| + (2^-16 + T 2^-22) sum |dy x|.  With one token that is one
+rounding of the exact result, where a rounding of q s on the way would add
+another u; over many tokens the error's norm is that of rounding the exact
+result.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import anima_flat_b200 as afb
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+U = {BF: 2.0**-8, HF: 2.0**-11}
+TINY = {BF: 2.0**-133, HF: 2.0**-25}
+
+
+def _codes(g, T, K):
+    q = torch.randint(-127, 128, (T, K), dtype=torch.int8, device="cuda", generator=g)
+    q[:, 0] = 127
+    return q
+
+
+def _check_wgrad(dy, q, s, T):
+    dw = afb.int8_wgrad(dy, q, s)
+    x = q.double() * s.double()
+    want, mag = dy.double().t() @ x, dy.double().abs().t() @ x.abs()
+    tol = U[dy.dtype] * want.abs() + (2.0**-16 + T * 2.0**-22) * mag + TINY[dy.dtype]
+    assert torch.isfinite(dw).all()
+    err = (dw.double() - want).abs()
+    assert (err <= tol).all(), f"{int((err > tol).sum())} of {err.numel()} off, worst {(err / tol).max():.3g}"
+    return dw, want
+
+
+# adapters' columns, padded rows, one tile of 128 columns, single tiles, clusters and pairs
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("T,N,K", [(1, 4, 144), (1, 16, 2048), (2, 17, 272), (1, 64, 256), (3, 100, 272), (1, 128, 528),
+                                   (1, 300, 1040), (1, 4096, 2048), (2, 4001, 2064), (70, 16, 8192), (66, 4096, 512)])
+def test_wgrad_rounds_once(T, N, K, dt, cuda_dev):
+    g = torch.Generator(device="cuda").manual_seed(T + N + K)
+    s = 2.0**-7 * (0.5 + torch.rand(T, 1, device="cuda", generator=g))
+    dy = (0.1 * torch.randn(T, N, device="cuda", generator=g)).to(dt)
+    _check_wgrad(dy, _codes(g, T, K), s, T)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("T,N,K", [(512, 16, 2048), (1000, 64, 528), (512, 128, 1024), (700, 2048, 2048), (512, 1000, 1040)])
+def test_wgrad_error_is_that_of_rounding_the_result(T, N, K, dt, cuda_dev):
+    g = torch.Generator(device="cuda").manual_seed(T + N)
+    s = 2.0**-7 * (0.5 + torch.rand(T, 1, device="cuda", generator=g))
+    dy = (0.1 * torch.randn(T, N, device="cuda", generator=g)).to(dt)
+    dw, want = _check_wgrad(dy, _codes(g, T, K), s, T)
+    # a rounding of q s would add an error of the same size: 1.41 times the norm
+    assert (dw.double() - want).norm() <= 1.1 * (want.to(dt).double() - want).norm()
+
+
+@pytest.mark.parametrize("N", [16, 64, 128, 1030, 4096])
+@pytest.mark.parametrize("top", [1e5, 1e-5, 1e-9])
+def test_wgrad_fp16_beside_codes_of_any_range(N, top, cuda_dev):
+    """Rows whose largest value fp16 does not hold, or holds in a few bits, as codes with fp32 scales do."""
+    T, K = 130, 512
+    g = torch.Generator(device="cuda").manual_seed(N)
+    s = (top / 127.0) * (0.5 + torch.rand(T, 1, device="cuda", generator=g))
+    dy = ((1e-3 if top > 1 else 1e3) * torch.randn(T, N, device="cuda", generator=g)).to(HF)
+    _check_wgrad(dy, _codes(g, T, K), s, T)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("N", [16, 100, 4096])
+def test_wgrad_infinities_and_nans_stay_what_they_are(N, dt, cuda_dev):
+    T, K = 70, 512
+    g = torch.Generator(device="cuda").manual_seed(N)
+    q, s = _codes(g, T, K), torch.rand(T, 1, device="cuda", generator=g) + 0.5
+    q[3, 5] = 0
+    dy = torch.randn(T, N, device="cuda", generator=g).to(dt)
+    dy[3, 1], dy[9, 2], dy[11, 3] = float("inf"), float("-inf"), float("nan")
+    dw, want = afb.int8_wgrad(dy, q, s).double(), dy.double().t() @ (q.double() * s.double())
+    assert torch.equal(torch.isnan(dw), torch.isnan(want)) and torch.isnan(want[1, 5])
+    assert torch.equal(torch.isinf(dw).logical_and(dw > 0), torch.isinf(want).logical_and(want > 0))
+    assert torch.equal(torch.isinf(dw).logical_and(dw < 0), torch.isinf(want).logical_and(want < 0))
