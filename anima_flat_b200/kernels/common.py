@@ -81,13 +81,15 @@ _Tensor, _Parameter = torch.Tensor, torch.nn.Parameter
 def _plain(*ts: torch.Tensor | None) -> bool:
     """True where the launches may be called directly, without torch's dispatcher.
 
-    That is: ordinary tensors, outside compilation, dispatch modes (fake tensors,
-    tracing), function transforms and forward-mode differentiation, all of which
-    need the registered op.  A Python custom op costs about 40 us a call, several
+    That is: ordinary tensors, outside compilation, ``torch.jit.trace``, dispatch
+    modes (fake tensors, graph capture), function transforms and forward-mode
+    differentiation, all of which need the registered op: none of them sees a
+    launch that goes by addresses.  A Python custom op costs about 40 us a call, several
     times a small launch; the direct call about 6.
     """
     if (
         torch.compiler.is_compiling()
+        or torch._C._is_tracing()
         or torch._C._len_torch_dispatch_stack()
         or torch._C._functorch.peek_interpreter_stack() is not None
         or torch.autograd.forward_ad._current_level >= 0

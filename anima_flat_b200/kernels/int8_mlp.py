@@ -42,19 +42,25 @@ class LoRA(NamedTuple):
     b: torch.Tensor
 
 
+def _forward(x, a1, b1, a2, b2, w1, w2, scaling):
+    """The output, and the activations that the backward pass reads."""
+    rows = x.reshape(-1, x.shape[-1])
+    q, s = rowquant_int8(rows)
+    t1 = rows @ a1.t()
+    h = int8_linear((q, s), w1, dtype=x.dtype).addmm_(t1, b1.t(), alpha=scaling)
+    gq, gs, c, cs = gelu_int8(h)
+    t2 = int8_restore(gq, gs, x.dtype) @ a2.t()
+    y = int8_linear((gq, gs), w2, dtype=x.dtype).addmm_(t2, b2.t(), alpha=scaling)
+    return y.view(*x.shape[:-1], y.shape[-1]), (q, s, c, cs, gq, gs, t1, t2)
+
+
 class _MlpFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a1, b1, a2, b2, w1, w2, scaling):
-        rows = x.reshape(-1, x.shape[-1])
-        q, s = rowquant_int8(rows)
-        t1 = rows @ a1.t()
-        h = int8_linear((q, s), w1, dtype=x.dtype).addmm_(t1, b1.t(), alpha=scaling)
-        gq, gs, c, cs = gelu_int8(h)
-        t2 = int8_restore(gq, gs, x.dtype) @ a2.t()
-        y = int8_linear((gq, gs), w2, dtype=x.dtype).addmm_(t2, b2.t(), alpha=scaling)
-        ctx.save_for_backward(q, s, c, cs, gq, gs, t1, t2, a1, b1, a2, b2, *w1, *w2)
+        y, kept = _forward(x, a1, b1, a2, b2, w1, w2, scaling)
+        ctx.save_for_backward(*kept, a1, b1, a2, b2, *w1, *w2)
         ctx.scaling = scaling
-        return y.view(*x.shape[:-1], y.shape[-1])
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -96,6 +102,7 @@ def int8_lora_mlp(
     Raises:
         ValueError: On tensors off CUDA, weights without transposed codes, or
             unsupported dtypes or shapes.
+        RuntimeError: Inside ``torch.jit.trace`` where a gradient is asked for.
     """
     _check_same_device(x, *up, *down, *lora_up, *lora_down)
     for name, w, lora, K in (("up", up, lora_up, x.shape[-1]), ("down", down, lora_down, up.q.shape[0])):
@@ -107,4 +114,9 @@ def int8_lora_mlp(
         if lora.a.shape != (r, K) or lora.b.shape != (N, r) or lora.a.dtype != x.dtype or lora.b.dtype != x.dtype:
             raise ValueError(f"lora_{name} must be {x.dtype} [r, {K}] and [{N}, r], got "
                              f"{lora.a.dtype} {list(lora.a.shape)} and {lora.b.dtype} {list(lora.b.shape)}")
-    return _MlpFn.apply(x, lora_up.a, lora_up.b, lora_down.a, lora_down.b, up, down, float(scaling))
+    args = (x, *lora_up, *lora_down, up, down, float(scaling))
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in args[:5]):
+        return _forward(*args)[0]
+    if torch.jit.is_tracing():
+        raise RuntimeError("int8_lora_mlp has no traced backward pass: trace it under torch.no_grad()")
+    return _MlpFn.apply(*args)
