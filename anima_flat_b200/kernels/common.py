@@ -65,11 +65,9 @@ def _check_same_device(*ts: torch.Tensor | None) -> None:
 def _dense(t: torch.Tensor) -> torch.Tensor:
     """Contiguous and 16-byte aligned: a copy only where `t` is not.
 
-    While code is being compiled there is no address to look at; the registered
-    ops call this again on what they are given.
+    It reads the tensor's address, so a public function calls it once `_plain`
+    has said that there is one; the registered ops call it on what they are given.
     """
-    if torch.compiler.is_compiling():
-        return t.contiguous()
     if t.is_contiguous():
         return t if not t.data_ptr() & 15 else t.clone()
     return t.contiguous()
@@ -99,6 +97,22 @@ def _plain(*ts: torch.Tensor | None) -> bool:
         if t is not None and type(t) is not _Tensor and type(t) is not _Parameter:
             return False
     return True
+
+
+def _registered(op, *args):
+    """Call a registered op where `_plain` has ruled the direct launch out.
+
+    The ops have no forward-mode derivative, which the dispatcher would leave
+    out in silence, and none under ``torch.func``'s gradients: both are refused.
+    """
+    if not torch.compiler.is_compiling():
+        ts = [a for a in args if isinstance(a, torch.Tensor) and a.is_floating_point()]
+        forward_ad = torch.autograd.forward_ad
+        if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+            raise RuntimeError(f"{op._qualname} has no forward-mode derivative")
+        if torch._C._functorch.peek_interpreter_stack() is not None and any(t.requires_grad for t in ts):
+            raise RuntimeError(f"{op._qualname} has no gradient under torch.func transforms: use torch.autograd")
+    return op(*args)
 
 
 _entries: dict[str, object] = {}

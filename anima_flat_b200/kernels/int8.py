@@ -29,7 +29,7 @@ from typing import NamedTuple
 import torch
 
 from .._lib import load
-from .common import HALF_TYPES, _check_half, _check_same_device, _dense, _launch, _plain
+from .common import HALF_TYPES, _check_half, _check_same_device, _dense, _launch, _plain, _registered
 
 __all__ = [
     "Int8Weight",
@@ -144,7 +144,9 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return _linear_bwd(dy, *ctx.saved_tensors), None, None, None, None
+        ws, wqt = ctx.saved_tensors
+        dx = _linear_bwd(dy, ws, wqt) if _plain(dy) else _registered(_int8_linear_bwd, dy, ws, wqt)
+        return dx, None, None, None, None
 
 
 # ----------------------------------------------------------------- custom ops --
@@ -163,7 +165,7 @@ def _int8_linear_codes(
     q: torch.Tensor, s: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias: torch.Tensor | None,
     dtype: torch.dtype,
 ) -> torch.Tensor:
-    return _product(_dense(q), s, _dense(wq), ws, bias, dtype)
+    return _product(_dense(q), _dense(s), _dense(wq), _dense(ws), bias, dtype)
 
 
 @_int8_linear_codes.register_fake
@@ -176,7 +178,7 @@ def _int8_linear(
     x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, wqt: torch.Tensor | None,
     bias: torch.Tensor | None,
 ) -> torch.Tensor:
-    return _linear(_dense(x), _dense(wq), ws, wqt, bias)
+    return _linear(_dense(x), _dense(wq), _dense(ws), wqt, bias)
 
 
 @_int8_linear.register_fake
@@ -223,7 +225,7 @@ def _(x):
 
 @torch.library.custom_op("anima_flat_b200::gelu_int8_bwd", mutates_args=())
 def _gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.Tensor:
-    return _gelu_bwd(_dense(dy), _dense(c), cs)
+    return _gelu_bwd(_dense(dy), _dense(c), _dense(cs))
 
 
 @_gelu_int8_bwd.register_fake
@@ -233,7 +235,7 @@ def _(dy, c, cs):
 
 @torch.library.custom_op("anima_flat_b200::int8_restore", mutates_args=())
 def _int8_restore(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    return _restore(_dense(q), s, dtype)
+    return _restore(_dense(q), _dense(s), dtype)
 
 
 @_int8_restore.register_fake
@@ -243,7 +245,7 @@ def _(q, s, dtype):
 
 @torch.library.custom_op("anima_flat_b200::int8_wgrad", mutates_args=())
 def _int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
-    return _wgrad(_dense(dy), _dense(q), s)
+    return _wgrad(_dense(dy), _dense(q), _dense(s))
 
 
 @_int8_wgrad.register_fake
@@ -297,8 +299,7 @@ def rowquant_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     _check_same_device(x)
     _check_half("x", x)
     _check_cols("x", x)
-    x = _dense(x)
-    return _quant(x) if _plain(x) else _rowquant_int8(x)
+    return _quant(_dense(x)) if _plain(x) else _registered(_rowquant_int8, x)
 
 
 def quantize_weight_int8(w: torch.Tensor, backward: bool = False) -> Int8Weight:
@@ -352,14 +353,13 @@ def int8_linear(
         if dtype not in HALF_TYPES:
             raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
         bias = _check_weight(wq, ws, bias, q.shape[-1], dtype)
-        q, s, wq, ws = _dense(q), s.contiguous(), _dense(wq), ws.contiguous()
-        product = _product if _plain(q, s, wq, ws, bias) else _int8_linear_codes
-        return product(q, s, wq, ws, bias, dtype)
+        if not _plain(q, s, wq, ws, bias):
+            return _registered(_int8_linear_codes, q, s, wq, ws, bias, dtype)
+        return _product(_dense(q), _dense(s), _dense(wq), _dense(ws), bias, dtype)
     _check_same_device(x, wq, ws, wqt, bias)
     _check_half("x", x)
     _check_cols("x", x)
     bias = _check_weight(wq, ws, bias, x.shape[-1], x.dtype)
-    x, wq, ws = _dense(x), _dense(wq), _dense(ws)
     grad = x.requires_grad and torch.is_grad_enabled()
     if grad:
         if wqt is None:
@@ -367,10 +367,10 @@ def int8_linear(
         if wqt.dtype != I8 or wqt.shape != (x.shape[-1], wq.shape[0]):
             raise ValueError(f"the transposed codes must be torch.int8 [{x.shape[-1]}, {wq.shape[0]}]")
         _check_cols("the transposed weight", wqt)
-        wqt = _dense(wqt)
     if not _plain(x, wq, ws, wqt, bias):
-        return _int8_linear(x, wq, ws, wqt, bias)
-    return _LinearFn.apply(x, wq, ws, wqt, bias) if grad else _linear(x, wq, ws, wqt, bias)
+        return _registered(_int8_linear, x, wq, ws, wqt, bias)
+    x, wq, ws = _dense(x), _dense(wq), _dense(ws)
+    return _LinearFn.apply(x, wq, ws, _dense(wqt), bias) if grad else _linear(x, wq, ws, wqt, bias)
 
 
 def int8_linear_dx(dy: torch.Tensor, weight: Int8Weight) -> torch.Tensor:
@@ -400,8 +400,9 @@ def int8_linear_dx(dy: torch.Tensor, weight: Int8Weight) -> torch.Tensor:
     N = dy.shape[-1]
     if wqt.dtype != I8 or wqt.ndim != 2 or wqt.shape[1] != N or ws.dtype != F32 or ws.numel() != N:
         raise ValueError(f"the transposed codes must be torch.int8 [K, {N}] with torch.float32 scales [{N}]")
-    dy, ws, wqt = _dense(dy), _dense(ws), _dense(wqt)
-    return _linear_bwd(dy, ws, wqt) if _plain(dy, ws, wqt) else _int8_linear_bwd(dy, ws, wqt)
+    if not _plain(dy, ws, wqt):
+        return _registered(_int8_linear_bwd, dy, ws, wqt)
+    return _linear_bwd(dy, _dense(ws), _dense(wqt))
 
 
 def gelu_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -420,8 +421,7 @@ def gelu_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor
     _check_same_device(x)
     _check_half("x", x)
     _check_cols("x", x)
-    x = _dense(x)
-    return _gelu(x) if _plain(x) else _gelu_int8(x)
+    return _gelu(_dense(x)) if _plain(x) else _registered(_gelu_int8, x)
 
 
 def gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.Tensor:
@@ -440,8 +440,9 @@ def gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.
     _check_codes(c, cs)
     if dy.shape != c.shape:
         raise ValueError(f"dy and the codes must match, got {list(dy.shape)} and {list(c.shape)}")
-    dy, c, cs = _dense(dy), _dense(c), cs.contiguous()
-    return _gelu_bwd(dy, c, cs) if _plain(dy, c, cs) else _gelu_int8_bwd(dy, c, cs)
+    if not _plain(dy, c, cs):
+        return _registered(_gelu_int8_bwd, dy, c, cs)
+    return _gelu_bwd(_dense(dy), _dense(c), _dense(cs))
 
 
 def int8_restore(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -454,8 +455,7 @@ def int8_restore(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bf
     _check_codes(q, s)
     if dtype not in HALF_TYPES:
         raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
-    q, s = _dense(q), s.contiguous()
-    return _restore(q, s, dtype) if _plain(q, s) else _int8_restore(q, s, dtype)
+    return _restore(_dense(q), _dense(s), dtype) if _plain(q, s) else _registered(_int8_restore, q, s, dtype)
 
 
 def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
@@ -479,5 +479,4 @@ def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tens
     _check_codes(q, s)
     if dy.shape[:-1] != q.shape[:-1] or not dy.shape[-1]:
         raise ValueError(f"dy and the codes must have the same tokens, got {list(dy.shape)} and {list(q.shape)}")
-    dy, q, s = _dense(dy), _dense(q), s.contiguous()
-    return _wgrad(dy, q, s) if _plain(dy, q, s) else _int8_wgrad(dy, q, s)
+    return _wgrad(_dense(dy), _dense(q), _dense(s)) if _plain(dy, q, s) else _registered(_int8_wgrad, dy, q, s)

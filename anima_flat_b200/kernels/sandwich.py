@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from .._lib import load
-from .common import HALF_TYPES, _check_half, _check_same_device, _check_vec, _dense, _launch, _plain
+from .common import HALF_TYPES, _check_half, _check_same_device, _check_vec, _dense, _launch, _plain, _registered
 
 __all__ = ["sandwich_norm", "sandwich_norm_bwd", "sandwich_norm_int8"]
 
@@ -82,8 +82,7 @@ def _saved(ctx, x, gate, post_weight, pre_weight, shift, scale, z, residual_scal
 def _grads(ctx, bwd, gh, gz):
     x, gate, post_weight, pre_weight, scale, z = ctx.saved_tensors
     dx, dres, dgate, dpost, dpre, dshift, dscale = bwd(
-        _dense(gh), None if gz is None else _dense(gz), z, x, gate, post_weight, pre_weight, scale,
-        ctx.residual_scale, ctx.eps)
+        gh, gz, z, x, gate, post_weight, pre_weight, scale, ctx.residual_scale, ctx.eps)
     return (dx, dres, dgate if gate is not None else None, dpost, dpre, dshift if ctx.has_shift else None,
             dscale if scale is not None else None, None, None)
 
@@ -100,7 +99,9 @@ class _SandwichFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gh, gz):
-        return _grads(ctx, _bwd, gh, gz)
+        if not _plain(gh, gz):
+            return _grads(ctx, lambda *args: _registered(_sandwich_norm_bwd, *args), gh, gz)
+        return _grads(ctx, _bwd, *_dense_all(gh, gz))
 
 
 # ----------------------------------------------------------------- custom ops --
@@ -165,10 +166,10 @@ torch.library.register_autograd("anima_flat_b200::sandwich_norm", _backward, set
 # --------------------------------------------------------------------- public --
 def _weight(w: torch.Tensor, D: int, name: str) -> torch.Tensor:
     if w.dtype is F32 and w.shape == (D,):
-        return _dense(w)
+        return w
     if w.numel() != D:
         raise ValueError(f"{name} must be [{D}], got {list(w.shape)}")
-    return _dense(w.to(F32).reshape(D))
+    return w.to(F32).reshape(D)
 
 
 def _vec(v: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype, name: str) -> torch.Tensor | None:
@@ -177,9 +178,9 @@ def _vec(v: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype, nam
     if v.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {v.dtype}")
     if v.shape == shape:
-        return _dense(v)
+        return v
     _check_vec(v, *shape, name)
-    return _dense(v.reshape(shape))
+    return v.reshape(shape)
 
 
 def _check_rows(x: torch.Tensor, *like: tuple[str, torch.Tensor | None]) -> tuple[int, int]:
@@ -199,7 +200,7 @@ def _check_rows(x: torch.Tensor, *like: tuple[str, torch.Tensor | None]) -> tupl
 def _args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps):
     _check_same_device(x, residual, gate, post_weight, pre_weight, shift, scale)
     vec, dtype = _check_rows(x, ("residual", residual)), x.dtype
-    return (_dense(x), _dense(residual), _vec(gate, vec, dtype, "gate"), _weight(post_weight, vec[1], "post_weight"),
+    return (x, residual, _vec(gate, vec, dtype, "gate"), _weight(post_weight, vec[1], "post_weight"),
             _weight(pre_weight, vec[1], "pre_weight"), _vec(shift, vec, dtype, "shift"),
             _vec(scale, vec, dtype, "scale"), float(residual_scale), float(eps))
 
@@ -228,7 +229,8 @@ def sandwich_norm(x, residual, gate, post_weight, pre_weight, shift=None, scale=
     """
     args = _args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
     if not _plain(*args[:7]):
-        return _sandwich_norm(*args)
+        return _registered(_sandwich_norm, *args)
+    args = (*_dense_all(*args[:7]), *args[7:])
     if torch.is_grad_enabled():
         for t in args[:7]:
             if t is not None and t.requires_grad:
@@ -251,7 +253,9 @@ def sandwich_norm_int8(x, residual, gate, post_weight, pre_weight, shift=None, s
         ValueError: On tensors off CUDA or unsupported dtypes or shapes.
     """
     args = _args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
-    return (_fwd_int8 if _plain(*args[:7]) else _sandwich_norm_int8)(*args)
+    if not _plain(*args[:7]):
+        return _registered(_sandwich_norm_int8, *args)
+    return _fwd_int8(*_dense_all(*args[:7]), *args[7:])
 
 
 def sandwich_norm_bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale=None, residual_scale=1.0, eps=1e-6):
@@ -276,7 +280,9 @@ def sandwich_norm_bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale=None, r
     """
     _check_same_device(gh, gz, z, x, gate, post_weight, pre_weight, scale)
     vec, dtype = _check_rows(z, ("x", x), ("gh", gh), ("gz", gz)), z.dtype
-    args = (_dense(gh), None if gz is None else _dense(gz), _dense(z), _dense(x), _vec(gate, vec, dtype, "gate"),
+    args = (gh, gz, z, x, _vec(gate, vec, dtype, "gate"),
             _weight(post_weight, vec[1], "post_weight"), _weight(pre_weight, vec[1], "pre_weight"),
             _vec(scale, vec, dtype, "scale"), float(residual_scale), float(eps))
-    return (_bwd if _plain(*args[:8]) else _sandwich_norm_bwd)(*args)
+    if not _plain(*args[:8]):
+        return _registered(_sandwich_norm_bwd, *args)
+    return _bwd(*_dense_all(*args[:8]), *args[8:])

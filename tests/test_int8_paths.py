@@ -2,9 +2,12 @@
 
 from __future__ import annotations
 
+import warnings
+
 import pytest
 import torch
 
+import anima_flat_b200 as afb
 from anima_flat_b200.kernels.common import _plain
 
 
@@ -14,3 +17,26 @@ def test_tracing_takes_the_registered_ops():
     x = torch.zeros(2, 16)
     torch.jit.trace(lambda t: (seen.append(_plain(t)), t + 1)[1], (x,), check_trace=False)
     assert seen == [False] and _plain(x)
+
+
+def test_fake_tensors_have_no_address_that_is_read():
+    """The public functions under FakeTensorMode, on fake CUDA tensors."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    bf, f32, i8 = torch.bfloat16, torch.float32, torch.int8
+    with FakeTensorMode(), warnings.catch_warnings():
+        warnings.simplefilter("error")
+        e = lambda *s, d=bf: torch.empty(*s, dtype=d, device="cuda")  # noqa: E731
+        x, dy, q, s = e(2, 6, 64), e(2, 6, 48), e(2, 6, 64, d=i8), e(12, 1, d=f32)
+        up = afb.Int8Weight(e(48, 64, d=i8), e(48, d=f32), e(64, 48, d=i8))
+        down = afb.Int8Weight(e(64, 48, d=i8), e(64, d=f32), e(48, 64, d=i8))
+        w, g = e(64, d=f32), e(2, 64)
+        shapes = [tuple(t.shape) for t in (
+            *afb.rowquant_int8(x), afb.int8_linear(x, up), afb.int8_linear((q, s), up), afb.int8_linear_dx(dy, up),
+            *afb.gelu_int8(x), afb.gelu_int8_bwd(x, q, s), afb.int8_restore(q, s), afb.int8_wgrad(dy, q, s),
+            *afb.sandwich_norm(x, x, g, w, w), *afb.sandwich_norm_int8(x, x, g, w, w),
+            *afb.sandwich_norm_bwd(x, None, x, x, g, w, w),
+            afb.int8_lora_mlp(x, up, down, afb.LoRA(e(4, 64), e(48, 4)), afb.LoRA(e(4, 48), e(64, 4))))]
+    rows, x, y = (12, 1), (2, 6, 64), (2, 6, 48)
+    assert shapes == [x, rows, y, y, x, x, rows, x, rows, x, x, (48, 64), x, x, x, rows, x,
+                      x, x, (2, 64), (64,), (64,), (2, 64), (2, 64), x]
