@@ -99,6 +99,19 @@ def _plain(*ts: torch.Tensor | None) -> bool:
     return True
 
 
+def _direct(*ts: torch.Tensor | None) -> bool:
+    """`_plain` for the ops without a gradient: false where one is asked of them too.
+
+    The registered op then keeps the graph, and the backward pass raises an error
+    where the direct call would have cut the gradient off in silence.
+    """
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return False
+    return _plain(*ts)
+
+
 def _registered(op, *args):
     """Call a registered op where `_plain` has ruled the direct launch out.
 

@@ -20,6 +20,9 @@ gradient (of a full weight, or of a low-rank adapter's first factor) straight
 from them, ``int8_restore`` gives the values back, and ``gelu_int8`` emits the
 codes of GELU(x) for the next product together with those of x, from which
 ``gelu_int8_bwd`` forms the activation's gradient.
+
+``int8_linear`` of a tensor is differentiable in it.  The other functions have no
+gradient: results of inputs that require one raise an error in a backward pass.
 """
 
 from __future__ import annotations
@@ -29,7 +32,7 @@ from typing import NamedTuple
 import torch
 
 from .._lib import load
-from .common import HALF_TYPES, _check_half, _check_same_device, _dense, _launch, _plain, _registered
+from .common import HALF_TYPES, _check_half, _check_same_device, _dense, _direct, _launch, _plain, _registered
 
 __all__ = [
     "Int8Weight",
@@ -274,6 +277,8 @@ def _check_weight(wq, ws, bias, K: int, dtype: torch.dtype) -> torch.Tensor | No
     N = wq.shape[0]
     if ws.dtype != F32 or ws.numel() != N:
         raise ValueError(f"the weight's scales must be torch.float32 [{N}], got {ws.dtype} {list(ws.shape)}")
+    if ws.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the weight's scales are constants here: they must not require a gradient")
     if bias is None:
         return None
     if bias.dtype != dtype or bias.numel() != N:
@@ -299,7 +304,7 @@ def rowquant_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     _check_same_device(x)
     _check_half("x", x)
     _check_cols("x", x)
-    return _quant(_dense(x)) if _plain(x) else _registered(_rowquant_int8, x)
+    return _quant(_dense(x)) if _direct(x) else _registered(_rowquant_int8, x)
 
 
 def quantize_weight_int8(w: torch.Tensor, backward: bool = False) -> Int8Weight:
@@ -342,8 +347,8 @@ def int8_linear(
         ``[..., N]``.
 
     Raises:
-        ValueError: On tensors off CUDA, unsupported dtypes or shapes, a bias that
-            requires a gradient, or an ``x`` that does without transposed codes.
+        ValueError: On tensors off CUDA, unsupported dtypes or shapes, a bias or
+            scales of the weight that require a gradient, or an ``x`` that does without transposed codes.
     """
     wq, ws, wqt = weight
     if not isinstance(x, torch.Tensor):
@@ -353,7 +358,7 @@ def int8_linear(
         if dtype not in HALF_TYPES:
             raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
         bias = _check_weight(wq, ws, bias, q.shape[-1], dtype)
-        if not _plain(q, s, wq, ws, bias):
+        if not _direct(q, s, wq, ws, bias):
             return _registered(_int8_linear_codes, q, s, wq, ws, bias, dtype)
         return _product(_dense(q), _dense(s), _dense(wq), _dense(ws), bias, dtype)
     _check_same_device(x, wq, ws, wqt, bias)
@@ -400,7 +405,7 @@ def int8_linear_dx(dy: torch.Tensor, weight: Int8Weight) -> torch.Tensor:
     N = dy.shape[-1]
     if wqt.dtype != I8 or wqt.ndim != 2 or wqt.shape[1] != N or ws.dtype != F32 or ws.numel() != N:
         raise ValueError(f"the transposed codes must be torch.int8 [K, {N}] with torch.float32 scales [{N}]")
-    if not _plain(dy, ws, wqt):
+    if not _direct(dy, ws, wqt):
         return _registered(_int8_linear_bwd, dy, ws, wqt)
     return _linear_bwd(dy, _dense(ws), _dense(wqt))
 
@@ -421,7 +426,7 @@ def gelu_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor
     _check_same_device(x)
     _check_half("x", x)
     _check_cols("x", x)
-    return _gelu(_dense(x)) if _plain(x) else _registered(_gelu_int8, x)
+    return _gelu(_dense(x)) if _direct(x) else _registered(_gelu_int8, x)
 
 
 def gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.Tensor:
@@ -440,7 +445,7 @@ def gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch.
     _check_codes(c, cs)
     if dy.shape != c.shape:
         raise ValueError(f"dy and the codes must match, got {list(dy.shape)} and {list(c.shape)}")
-    if not _plain(dy, c, cs):
+    if not _direct(dy, c, cs):
         return _registered(_gelu_int8_bwd, dy, c, cs)
     return _gelu_bwd(_dense(dy), _dense(c), _dense(cs))
 
@@ -455,7 +460,7 @@ def int8_restore(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype = torch.bf
     _check_codes(q, s)
     if dtype not in HALF_TYPES:
         raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
-    return _restore(_dense(q), _dense(s), dtype) if _plain(q, s) else _registered(_int8_restore, q, s, dtype)
+    return _restore(_dense(q), _dense(s), dtype) if _direct(q, s) else _registered(_int8_restore, q, s, dtype)
 
 
 def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
@@ -479,4 +484,4 @@ def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tens
     _check_codes(q, s)
     if dy.shape[:-1] != q.shape[:-1] or not dy.shape[-1]:
         raise ValueError(f"dy and the codes must have the same tokens, got {list(dy.shape)} and {list(q.shape)}")
-    return _wgrad(_dense(dy), _dense(q), _dense(s)) if _plain(dy, q, s) else _registered(_int8_wgrad, dy, q, s)
+    return _wgrad(_dense(dy), _dense(q), _dense(s)) if _direct(dy, q, s) else _registered(_int8_wgrad, dy, q, s)

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from .._lib import load
-from .common import HALF_TYPES, _check_half, _check_same_device, _check_vec, _dense, _launch, _plain, _registered
+from .common import HALF_TYPES, _check_half, _check_same_device, _check_vec, _dense, _direct, _launch, _plain, _registered
 
 __all__ = ["sandwich_norm", "sandwich_norm_bwd", "sandwich_norm_int8"]
 
@@ -242,8 +242,8 @@ def sandwich_norm_int8(x, residual, gate, post_weight, pre_weight, shift=None, s
                        eps=1e-6):
     """``sandwich_norm`` whose output h is returned as 8-bit codes with a scale per token.
 
-    Arguments as for ``sandwich_norm``; not differentiable (``sandwich_norm_bwd``
-    takes its z).
+    Arguments as for ``sandwich_norm``; not differentiable: a backward pass through
+    its results raises an error (``sandwich_norm_bwd`` takes its z).
 
     Returns:
         ``(q, s, z)``: codes ``[B, S, D]`` int8 and scales ``[B * S, 1]`` float32 of
@@ -253,7 +253,7 @@ def sandwich_norm_int8(x, residual, gate, post_weight, pre_weight, shift=None, s
         ValueError: On tensors off CUDA or unsupported dtypes or shapes.
     """
     args = _args(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps)
-    if not _plain(*args[:7]):
+    if not _direct(*args[:7]):
         return _registered(_sandwich_norm_int8, *args)
     return _fwd_int8(*_dense_all(*args[:7]), *args[7:])
 
@@ -283,6 +283,6 @@ def sandwich_norm_bwd(gh, gz, z, x, gate, post_weight, pre_weight, scale=None, r
     args = (gh, gz, z, x, _vec(gate, vec, dtype, "gate"),
             _weight(post_weight, vec[1], "post_weight"), _weight(pre_weight, vec[1], "pre_weight"),
             _vec(scale, vec, dtype, "scale"), float(residual_scale), float(eps))
-    if not _plain(*args[:8]):
+    if not _direct(*args[:8]):
         return _registered(_sandwich_norm_bwd, *args)
     return _bwd(*_dense_all(*args[:8]), *args[8:])
