@@ -93,6 +93,32 @@ rowquant_int8_kernel(const QuantArgs a) {
   }
 }
 
+// GELU of a pair (erf form), by Abramowitz & Stegun 7.1.26: with r = poly(t)
+// exp(-x^2 / 2), 1 - erf(|x| / sqrt 2) up to 1.5e-7,
+//   gelu(x) = max(x, 0) - |x| r / 2,
+// which nothing cancels below zero: there it is -|x| r / 2, within 2^-8 of GELU
+// down to -6 (r's relative error), where x / 2 (1 + erf) would keep a step of
+// 2^-24 |x|, more than GELU itself.  A row with nothing larger takes its scale and
+// codes from such values.
+__device__ __forceinline__ f2_t gelu2(f2_t x) {
+  constexpr f2_t kAbs = 0x7fffffff7fffffffull;
+  const f2_t hx = mul2(x, splat2(0.5f)), hax = hx & kAbs;
+  const f2_t den = fma2(hax, splat2(2.0f * (0.3275911f * 0.707106769084930419921875f)), splat2(1.0f));
+  float t0, t1, e0, e1;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(f2lo(den)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(f2hi(den)));
+  const f2_t t = f2(t0, t1);
+  f2_t n = fma2(splat2(-1.061405429f), t, splat2(1.453152027f));  // n = -poly(t)
+  n = fma2(n, t, splat2(-1.421413741f));
+  n = fma2(n, t, splat2(0.284496736f));
+  n = fma2(n, t, splat2(-0.254829592f));
+  n = mul2(n, t);
+  const f2_t arg = mul2(mul2(x, x), splat2(-0.721347520444481703680f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(f2lo(arg)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(f2hi(arg)));
+  return fma2(hax, mul2(n, f2(e0, e1)), add2(hx, hax));  // x / 2 + |x| / 2 is exact
+}
+
 // GELU and its input's codes.  |GELU| is at most 0.17 below zero and increases
 // above it, so from x = 0.34 on the row's largest |GELU| is that of its largest
 // x: the row's scale is known before any GELU is formed, and each is formed and
@@ -142,7 +168,7 @@ gelu_int8_kernel(const QuantArgs a) {
     }
   const uint32_t top = group_max(amax, 0);
   const float most = __uint_as_float(group_max(pmax, 1));
-  uint32_t gtop = __float_as_uint(f2lo(fast_gelu2(splat2(most))));
+  uint32_t gtop = __float_as_uint(f2lo(gelu2(splat2(most))));
   if (top >= 0x7f800000u) {
     gtop = top;
   } else if (most < 0.34f) {
@@ -150,7 +176,7 @@ gelu_int8_kernel(const QuantArgs a) {
 #pragma unroll
     for (int c = 0; c < CPL; ++c)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g = max_abs_nan(g, fast_gelu2(unpack2<DT>(word(xv[c][j >> 2], j & 3))));
+      for (int j = 0; j < 8; ++j) g = max_abs_nan(g, gelu2(unpack2<DT>(word(xv[c][j >> 2], j & 3))));
     gtop = group_max(g, 2);
   }
   if (!row_ok) return;
@@ -170,7 +196,7 @@ gelu_int8_kernel(const QuantArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         v[j] = unpack2<DT>(word(xv[c][h], j));
-        g[j] = fast_gelu2(v[j]);
+        g[j] = gelu2(v[j]);
       }
       q[h] = codes8<false>(g, rg);
       x[h] = codes8(v, rx);
@@ -183,8 +209,8 @@ gelu_int8_kernel(const QuantArgs a) {
 // Warps of a row's group and chunks of 16 a thread.  The plain forms take two
 // chunks a thread (one where 32 threads hold the row): 8192 rows of 8192 take
 // 31.8 us so, 40.5 with one, which waits on twice the warps.  GELU takes one up
-// to 8 warps (4096 x 2048: 10.0 us, 12.3 with two) and two from there on
-// (8192 x 8192: 61.9 us with 8 warps, 75.9 with 16).
+// to 8 warps (4096 x 2048: 10.2 us, 2.3 more with two) and two from there on
+// (8192 x 8192: 62.7 us with 8 warps, 14 more with 16).
 template <int MODE>
 static bool quant_shape(int64_t K, int* group, int* cpl) {
   const int64_t chunks = K / 16;

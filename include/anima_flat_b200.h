@@ -281,7 +281,8 @@ int afb_rms_silu_bwd(const void* s, const void* gamma, const void* dy, const voi
 int afb_rowquant_int8(const void* x, const void* cols, void* q, void* s, int64_t rows, int64_t K,
                       int dtype, void* stream);
 
-/* q, s: codes of GELU(x) (erf form, A&S 7.1.26); c, cs: codes of x, the
+/* q, s: codes of GELU(x) (erf form, A&S 7.1.26: within 2^-20 + 2^-12 |g|, and
+ * below zero within 2^-8 |g| down to -6); c, cs: codes of x, the
  * checkpoint that afb_gelu_int8_bwd reads. */
 int afb_gelu_int8(const void* x, void* q, void* s, void* c, void* cs, int64_t rows, int64_t K,
                   int dtype, void* stream);

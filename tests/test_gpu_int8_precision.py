@@ -8,6 +8,10 @@ it, and two products a token go into an fp32 sum, whose additions may cut off
 rounding of the exact result, where a rounding of q s on the way would add
 another u; over many tokens the error's norm is that of rounding the exact
 result.
+
+gelu_int8: below zero the error function's approximation (A&S 7.1.26) is within
+0.0036 of 1 + erf down to -6, and the special-function unit's exponential and
+reciprocal within 2^-16 there: 2^-8 of GELU in all.
 """
 
 from __future__ import annotations
@@ -86,3 +90,24 @@ def test_wgrad_infinities_and_nans_stay_what_they_are(N, dt, cuda_dev):
     assert torch.equal(torch.isnan(dw), torch.isnan(want)) and torch.isnan(want[1, 5])
     assert torch.equal(torch.isinf(dw).logical_and(dw > 0), torch.isinf(want).logical_and(want > 0))
     assert torch.equal(torch.isinf(dw).logical_and(dw < 0), torch.isinf(want).logical_and(want < 0))
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("K", [16, 528, 2048, 8192, 16384])
+def test_gelu_rows_far_below_zero(K, dt, cuda_dev):
+    """Rows whose largest |GELU| is small: scale and codes to a fraction of the row's own maximum."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = -4.0 - 2.0 * torch.rand(12, K, device="cuda", generator=g)
+    x[0], x[1], x[2] = -5.5, -6.0, -4.0
+    x[3] = -1.0 - 5.0 * torch.rand(K, device="cuda", generator=g)
+    x[4] = -6.0 * torch.rand(K, device="cuda", generator=g)
+    x[5] = x[4] * 2.0**-10
+    x[6, :8] = 0.0
+    x[7] = 0.33
+    x = x.to(dt).clamp_min(-6.0)
+    q, s, c, cs = afb.gelu_int8(x)
+    want = x.double() * torch.special.ndtr(x.double())
+    top = want.abs().amax(1, keepdim=True)
+    assert ((s.double() * 127.0 - top).abs() <= 2.0**-8 * top).all()
+    assert ((q.double() * s.double() - want).abs() <= 0.5001 * s.double() + 2.0**-8 * top).all()
+    assert q.abs().amax(1).eq(127).all()
