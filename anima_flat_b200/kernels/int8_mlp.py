@@ -10,6 +10,10 @@ step would:
 What the forward pass keeps for the backward pass is what the products read: the
 codes of x and of g, and the codes of h, one byte an element each, instead of
 three bf16 activations.  The adapters' small products are plain matrix products.
+
+Every product is summed in 32 bits or exactly and rounded once to the activations'
+type, t1, t2 and their gradients too, as separate layers of that type do; an
+adapter's part is added to the rounded product of its layer, and the sum rounded.
 """
 
 from __future__ import annotations
@@ -42,6 +46,11 @@ class LoRA(NamedTuple):
     b: torch.Tensor
 
 
+def _scaled_product(a, b, scaling):
+    """``scaling * (a @ b)``, rounded once."""
+    return a.new_empty((a.shape[0], b.shape[1])).addmm_(a, b, beta=0, alpha=scaling)
+
+
 def _forward(x, a1, b1, a2, b2, w1, w2, scaling):
     """The output, and the activations that the backward pass reads."""
     rows = x.reshape(-1, x.shape[-1])
@@ -69,12 +78,12 @@ class _MlpFn(torch.autograd.Function):
         w1, w2 = Int8Weight(*w[:3]), Int8Weight(*w[3:])
         shape = (*dy.shape[:-1], q.shape[-1])
         dy = dy.reshape(-1, dy.shape[-1])
-        dt2 = (dy @ b2).mul_(ctx.scaling)
-        db2 = (dy.t() @ t2).mul_(ctx.scaling)
+        dt2 = _scaled_product(dy, b2, ctx.scaling)
+        db2 = _scaled_product(dy.t(), t2, ctx.scaling)
         da2 = int8_wgrad(dt2, gq, gs)
         dh = gelu_int8_bwd(int8_linear_dx(dy, w2).addmm_(dt2, a2), c, cs)
-        dt1 = (dh @ b1).mul_(ctx.scaling)
-        db1 = (dh.t() @ t1).mul_(ctx.scaling)
+        dt1 = _scaled_product(dh, b1, ctx.scaling)
+        db1 = _scaled_product(dh.t(), t1, ctx.scaling)
         da1 = int8_wgrad(dt1, q, s)
         dx = int8_linear_dx(dh, w1).addmm_(dt1, a1).view(shape) if ctx.needs_input_grad[0] else None
         return dx, da1, db1, da2, db2, None, None, None

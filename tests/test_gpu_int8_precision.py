@@ -12,6 +12,10 @@ result.
 gelu_int8: below zero the error function's approximation (A&S 7.1.26) is within
 0.0036 of 1 + erf down to -6, and the special-function unit's exponential and
 reciprocal within 2^-16 there: 2^-8 of GELU in all.
+
+int8_lora_mlp: an adapter's gradients are products with the scaling, each rounded
+once from an fp32 sum: u |db| + T 2^-22 sum of magnitudes for b; for a over one
+token u of the inner gradient and u of the result.
 """
 
 from __future__ import annotations
@@ -111,3 +115,30 @@ def test_gelu_rows_far_below_zero(K, dt, cuda_dev):
     assert ((s.double() * 127.0 - top).abs() <= 2.0**-8 * top).all()
     assert ((q.double() * s.double() - want).abs() <= 0.5001 * s.double() + 2.0**-8 * top).all()
     assert q.abs().amax(1).eq(127).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("T", [1, 70])
+def test_adapter_gradients_round_once(T, dt, cuda_dev):
+    K, H, N, r, scaling = 256, 528, 272, 64, 1.0 / 3.0
+    g = torch.Generator(device="cuda").manual_seed(T)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    up = afb.quantize_weight_int8((rn(H, K) / K**0.5).to(dt), backward=True)
+    down = afb.quantize_weight_int8((rn(N, H) / H**0.5).to(dt), backward=True)
+    x, dy = rn(T, K).to(dt), rn(T, N).to(dt)
+    a1, b1, a2, b2 = (t.to(dt).requires_grad_(True) for t in (rn(r, K) / 16, rn(H, r) / 8, rn(r, H) / 16, rn(N, r) / 8))
+    y = afb.int8_lora_mlp(x, up, down, afb.LoRA(a1, b1), afb.LoRA(a2, b2), scaling)
+    da2, db2 = torch.autograd.grad(y, (a2, b2), dy)
+    with torch.no_grad():  # the inner values, as the forward pass has them
+        h = afb.int8_linear(afb.rowquant_int8(x), up, dtype=dt).addmm_(x @ a1.t(), b1.t(), alpha=scaling)
+        gq, gs, _, _ = afb.gelu_int8(h)
+        t2 = (afb.int8_restore(gq, gs, dt) @ a2.t()).double()
+    u, d = U[dt], dy.double()
+    want, mag = scaling * (d.t() @ t2), scaling * (d.t().abs() @ t2.abs())
+    assert ((db2.double() - want).abs() <= u * want.abs() + T * 2.0**-22 * mag + TINY[dt]).all()
+    if T == 1:
+        inner, imag = scaling * (d @ b2.double()), scaling * (d.abs() @ b2.double().abs())
+        v = gq.double() * gs.double()
+        want, mag = inner.t() @ v, imag.t() @ v.abs()
+        tol = u * want.abs() + (1 + u) * (u * want.abs() + N * 2.0**-23 * mag) + 2.0**-15 * want.abs() + TINY[dt]
+        assert ((da2.double() - want).abs() <= tol).all()
