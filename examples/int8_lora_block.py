@@ -6,7 +6,9 @@ scale, the norm before the next block), at this framework's model widths:
     y = MLP(h) with adapters         int8_lora_mlp
     h', z' = sandwich_norm(y, z)     and its codes when serving: sandwich_norm_int8
 
-The adapters learn a teacher's change of the block from synthetic tokens.
+The adapters learn a teacher's change of the block from synthetic tokens, and
+serving multiplies by them as trained: weights and activations between layers are
+codes, the adapters' small factors and products 16 bits wide.
 
     python examples/int8_lora_block.py [--tokens 4096] [--steps 30] [--rank 16]
 """
@@ -44,9 +46,15 @@ def run_block(p: dict, h: torch.Tensor, z: torch.Tensor) -> tuple[torch.Tensor, 
 
 
 def serve_block(p: dict, q: torch.Tensor, s: torch.Tensor, z: torch.Tensor):
-    """The block on codes, without adapters: codes in, codes out."""
-    gq, gs, _, _ = afb.gelu_int8(afb.int8_linear((q, s), p["up"]))
-    y = afb.int8_linear((gq, gs), p["down"])
+    """The block with its adapters on codes: codes in, codes out."""
+
+    def layer(q, s, weight, lora):
+        x = afb.int8_restore(q, s).flatten(0, 1)  # the adapter's first factor is 16 bits wide
+        y = afb.int8_linear((q.flatten(0, 1), s), weight).addmm_(x @ lora.a.t(), lora.b.t())
+        return y.view(*q.shape[:-1], -1)
+
+    gq, gs, _, _ = afb.gelu_int8(layer(q, s, p["up"], p["lora_up"]))
+    y = layer(gq, gs, p["down"], p["lora_down"])
     return afb.sandwich_norm_int8(y, z, p["gate"], p["post"], p["pre"], p["shift"], p["scale"])
 
 
