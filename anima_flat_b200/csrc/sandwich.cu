@@ -183,9 +183,7 @@ __global__ void __launch_bounds__((GROUP > 4 ? GROUP : 4) * 32) sandwich_fwd_ker
 // threads take four rows at a time.  A thread owns 8 columns and keeps their
 // factors in registers; in the kernel above every row reads them again, 14 bytes
 // an element from L1 for 8 from memory.  Bulk copies keep the next rows coming.
-// From 2^19 elements on for rows of 1024 and more (256 x 2048: 4.0 us against 4.2
-// above, 1024 x 2048: 5.5 against 6.5; 128 x 2048: 4.0 and 4.0), from 2^22 for
-// shorter ones (8192 x 512: 8.6 against 9.1; 2048 x 512: 4.4 against 3.6).
+// Which sizes: fwd_by_teams.
 constexpr int64_t kManyWide = 1 << 19, kManyNarrow = 1 << 22;
 constexpr int kFwdRows = 4;
 constexpr int kFwdStages = 3;
@@ -378,6 +376,28 @@ static int64_t rows_of_block(int64_t B, int64_t S, int64_t least) {
   return c > least ? c : least;
 }
 
+// Whether teams take a forward pass.  Where a block a multiprocessor holds all
+// samples: from 2^19 elements on for rows of 1024 and more (256 x 2048: 4.0 us
+// against 4.2 by groups of warps, 1024 x 2048: 5.5 against 6.5; 128 x 2048: 4.0 and
+// 4.0), from 2^22 for shorter ones (8192 x 512: 8.6 against 9.1; 2048 x 512: 4.4
+// against 3.6).  A block takes one sample's rows, so more samples are more blocks,
+// one after another, each with its start and its factors to load: by what was
+// measured, in ns, 2500 a round of 148 and 0.195 an element of a block (0.12 in a
+// round of few, and all 15% more for codes), where groups of warps take 2400 and
+// 0.002 an element in all (0.0016 in short rows).  4096 samples of one row of 2048: 93
+// us by teams, 21 by groups; 256 of 64: 45 and 67.
+static bool fwd_by_teams(int64_t B, int64_t S, int64_t D, bool int8) {
+  const int64_t all = B * S * D;
+  if (all < (D >= 1024 ? kManyWide : kManyNarrow)) return false;
+  const int64_t chunk = rows_of_block(B, S, teams_of(static_cast<int>(D)) * kFwdRows);
+  const int64_t blocks = B * ((S + chunk - 1) / chunk), rounds = blocks / 148, rest = blocks % 148;
+  if (blocks <= 148) return true;
+  const int64_t mine = (S < chunk ? S : chunk) * D;
+  const int64_t teams = rounds * (2500 + mine * 195 / 1000) + (rest ? 2500 + mine * (120 + 75 * rest / 148) / 1000 : 0);
+  const int64_t groups = 2400 + all * (D >= 1024 ? 20 : 16) / 10000;
+  return teams * (int8 ? 115 : 100) / 100 < groups;
+}
+
 template <bool INT8>
 static cudaError_t launch_rows(const SandwichArgs& a, int64_t B, int64_t S, int dtype, cudaStream_t st) {
   const int team = team_threads_of(a.D), teams = teams_of(a.D);
@@ -401,7 +421,7 @@ static cudaError_t launch_fwd_g(const SandwichArgs& a, int dtype, cudaStream_t s
 template <bool INT8>
 static cudaError_t launch_fwd(const SandwichArgs& a, int64_t B, int64_t S, int dtype, cudaStream_t st) {
   const int nv = a.D / 8;
-  if (a.rows * a.D >= (a.D >= 1024 ? kManyWide : kManyNarrow)) return launch_rows<INT8>(a, B, S, dtype, st);
+  if (fwd_by_teams(B, S, a.D, INT8)) return launch_rows<INT8>(a, B, S, dtype, st);
   if (nv <= 32) return launch_fwd_g<1, 1, INT8>(a, dtype, st);
   if (nv <= 64) return launch_fwd_g<2, 1, INT8>(a, dtype, st);
   if (nv <= 128) return launch_fwd_g<4, 1, INT8>(a, dtype, st);

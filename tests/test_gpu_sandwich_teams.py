@@ -44,3 +44,32 @@ def test_codes(B, S, D, cuda_dev):
     top = h.abs().amax(1, keepdim=True)
     _within(s, top / 127.0, err.amax(1, keepdim=True) / 127.0 + 2.0**-23 * top)
     _within(q.view(-1, D).double() * s.double(), h, 0.5001 * s.double() + 2 * err.amax(1, keepdim=True))
+
+
+def _time(fn):
+    """Milliseconds of 20 calls in a graph, the least of five."""
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        fn()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(20):
+            fn()
+    best = float("inf")
+    for _ in range(5):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+@pytest.mark.parametrize("fn", [afb.sandwich_norm, afb.sandwich_norm_int8])
+def test_short_samples_cost_what_their_rows_do(fn, cuda_dev):
+    """4096 rows of 4096 samples read 1.75 times the bytes of 4096 rows of one: no 4 times the time."""
+    times = [_time(lambda c=_case(B, S, 2048, BF, 1): _call(c, fn)) for B, S in ((1, 4096), (4096, 1))]
+    assert times[1] <= 4 * times[0]
