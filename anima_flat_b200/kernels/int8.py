@@ -233,7 +233,7 @@ def _gelu_int8_bwd(dy: torch.Tensor, c: torch.Tensor, cs: torch.Tensor) -> torch
 
 @_gelu_int8_bwd.register_fake
 def _(dy, c, cs):
-    return torch.empty_like(dy)
+    return dy.new_empty(dy.shape)
 
 
 @torch.library.custom_op("anima_flat_b200::int8_restore", mutates_args=())

@@ -116,7 +116,7 @@ def _sandwich_norm(
 
 @_sandwich_norm.register_fake
 def _(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps):
-    return torch.empty_like(x), torch.empty_like(x)
+    return x.new_empty(x.shape), x.new_empty(x.shape)
 
 
 @torch.library.custom_op("anima_flat_b200::sandwich_norm_int8", mutates_args=())
@@ -131,7 +131,7 @@ def _sandwich_norm_int8(
 @_sandwich_norm_int8.register_fake
 def _(x, residual, gate, post_weight, pre_weight, shift, scale, residual_scale, eps):
     B, S, _ = x.shape
-    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty((B * S, 1), dtype=F32), torch.empty_like(x)
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty((B * S, 1), dtype=F32), x.new_empty(x.shape)
 
 
 @torch.library.custom_op("anima_flat_b200::sandwich_norm_bwd", mutates_args=())
@@ -148,7 +148,7 @@ def _(gh, gz, z, x, gate, post_weight, pre_weight, scale, residual_scale, eps):
     B, _, D = z.shape
     vec = [z.new_empty((B, D)) for _ in range(3)]
     w = [z.new_empty(D, dtype=F32) for _ in range(2)]
-    return torch.empty_like(x), torch.empty_like(z), vec[0], w[0], w[1], vec[1], vec[2]
+    return x.new_empty(x.shape), z.new_empty(z.shape), vec[0], w[0], w[1], vec[1], vec[2]
 
 
 def _setup(ctx, inputs, output):

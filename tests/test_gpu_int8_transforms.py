@@ -95,3 +95,21 @@ def test_saved_tensors_on_the_host(cuda_dev):
         with torch.autograd.graph.save_on_cpu():
             out = fn(*leaves)
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, g), want, strict=True))
+
+
+@pytest.mark.parametrize("name", ["rowquant_int8", "int8_linear", "gelu_int8_bwd", "int8_wgrad", "sandwich_norm", "sandwich_norm_int8",
+                                  "sandwich_norm_bwd"])
+def test_compiled_code_with_permuted_inputs(name, cuda_dev):
+    """Strides and values of compiled code, the backward pass's too, on inputs that are not contiguous."""
+    fn, args = CALLS[name]
+    at = [t.transpose(0, 1).contiguous().transpose(0, 1) if t.ndim > 1 else t for t in args(_inputs(8))]
+    want = _list(fn(*at))
+    got = _list(torch.compile(lambda *ts: [t + 0 for t in _list(fn(*ts))], backend="aot_eager", fullgraph=True)(*at))
+    assert all(torch.equal(a, b) and a.stride() == b.stride() for a, b in zip(got, want, strict=True))
+    if name == "sandwich_norm":
+        grads = []
+        for f in (fn, torch.compile(fn, backend="aot_eager", fullgraph=True)):
+            leaves = [t.detach().requires_grad_(True) for t in at]
+            h, z = f(*leaves)
+            grads.append(torch.autograd.grad((h.float() * z.float()).sum(), leaves))
+        assert all(torch.equal(a, b) for a, b in zip(*grads))

@@ -40,3 +40,21 @@ def test_fake_tensors_have_no_address_that_is_read():
     rows, x, y = (12, 1), (2, 6, 64), (2, 6, 48)
     assert shapes == [x, rows, y, y, x, x, rows, x, rows, x, x, (48, 64), x, x, x, rows, x,
                       x, x, (2, 64), (64,), (64,), (2, 64), (2, 64), x]
+
+
+def test_outputs_are_contiguous_whatever_the_inputs_are():
+    """As the launches write them: what is compiled from the registered ops relies on their strides."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    ops = torch.ops.anima_flat_b200
+    with FakeTensorMode():
+        e = lambda *s, d=torch.bfloat16: torch.empty(*s, dtype=d, device="cuda").transpose(0, 1)  # noqa: E731
+        x, q, s, w = e(6, 2, 64), e(6, 2, 64, d=torch.int8), e(1, 12, d=torch.float32), torch.empty(64, device="cuda")
+        assert not x.is_contiguous()
+        wq, ws = e(64, 48, d=torch.int8), torch.empty(48, device="cuda")
+        outs = (*ops.rowquant_int8(x), ops.int8_linear(x, wq, ws, None, None), ops.int8_linear_codes(q, s, wq, ws, None, x.dtype),
+                ops.int8_linear_bwd(x, w, wq), *ops.gelu_int8(x), ops.gelu_int8_bwd(x, q, s), ops.int8_restore(q, s, x.dtype),
+                ops.int8_wgrad(x, q, s), *ops.sandwich_norm(x, x, None, w, w, None, None, 1.0, 1e-6),
+                *ops.sandwich_norm_int8(x, x, None, w, w, None, None, 1.0, 1e-6),
+                *ops.sandwich_norm_bwd(x, None, x, x, None, w, w, None, 1.0, 1e-6))
+        assert len(outs) == 24 and all(t.is_contiguous() for t in outs)
