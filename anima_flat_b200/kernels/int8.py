@@ -468,7 +468,7 @@ def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tens
 
     Args:
         dy: Gradient at the layer's output, shape ``[..., N]`` bf16 or fp16 (for a
-            low-rank adapter, at its first factor's output: N is the rank).
+            low-rank adapter, at its first factor's output: N is the rank), N at most 2^20.
         q: Codes of the layer's input, int8 ``[..., K]``, same leading sizes.
         s: Their scales, one per token.
 
@@ -484,4 +484,6 @@ def int8_wgrad(dy: torch.Tensor, q: torch.Tensor, s: torch.Tensor) -> torch.Tens
     _check_codes(q, s)
     if dy.shape[:-1] != q.shape[:-1] or not dy.shape[-1]:
         raise ValueError(f"dy and the codes must have the same tokens, got {list(dy.shape)} and {list(q.shape)}")
+    if dy.shape[-1] > 2**20:
+        raise ValueError(f"the last dimension of dy must be at most 2^20, got {dy.shape[-1]}")
     return _wgrad(_dense(dy), _dense(q), _dense(s)) if _direct(dy, q, s) else _registered(_int8_wgrad, dy, q, s)

@@ -191,6 +191,8 @@ def _check_rows(x: torch.Tensor, *like: tuple[str, torch.Tensor | None]) -> tupl
     D = shape[2]
     if D < 8 or D % 8 or D > 4096:
         raise ValueError(f"D must be a multiple of 8 in [8, 4096], got {D}")
+    if shape[0] > 65535 or shape[0] * shape[1] >= 2**31:
+        raise ValueError(f"B must be at most 65535 and B * S below 2^31, got {list(shape)}")
     for name, t in like:
         if t is not None and (t.shape != shape or t.dtype is not x.dtype):
             raise ValueError(f"{name} must be {x.dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
@@ -211,7 +213,8 @@ def sandwich_norm(x, residual, gate, post_weight, pre_weight, shift=None, scale=
     Differentiable in every tensor.
 
     Args:
-        x: The block's output, shape ``[B, S, D]`` bf16 or fp16, D a multiple of 8 up to 4096.
+        x: The block's output, shape ``[B, S, D]`` bf16 or fp16, D a multiple of 8 up to 4096,
+            B at most 65535.
         residual: Residual stream, same shape and dtype as ``x``.
         gate: Gate, shape ``[B, D]``, or None for one.
         post_weight: Weight ``[D]`` of the norm after the block.

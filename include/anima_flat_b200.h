@@ -311,7 +311,7 @@ int afb_int8_linear_x(const void* x, const void* cols, const void* w, const void
                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* dw[n, k] = sum_t dy[t, n] q[t, k] s[t], summed in fp32 in an order that the
- * sizes fix; dy s is held to 2^-16 of it, in the range of fp32 for either type.  dy [rows, N]; q [rows, K], K a multiple of 16 up to 2^20;
+ * sizes fix; dy s is held to 2^-16 of it, in the range of fp32 for either type.  dy [rows, N], N at most 2^20; q [rows, K], K a multiple of 16 up to 2^20;
  * s [rows]; dw [N, K] of `dtype` (zero where rows = 0).  Workspace as the query
  * says (none where N is a multiple of 8), 16-byte aligned, overwritten. */
 size_t afb_int8_wgrad_workspace(int64_t rows, int64_t N, int64_t K);
@@ -326,7 +326,8 @@ int afb_int8_wgrad(const void* dy, const void* q, const void* s, void* dw, int64
  *   h = rms(z) * pre_weight * scale + shift        (z as stored)
  * x, residual, h, z [batch, seq, dim] of `dtype` (0 bf16, 1 fp16); gate,
  * shift, scale [batch, dim] of `dtype`, each NULL for 1, 0, 1; post_weight,
- * pre_weight [dim] fp32.  dim a multiple of 8 up to 4096.  The _int8 form
+ * pre_weight [dim] fp32.  dim a multiple of 8 up to 4096, batch at
+ * most 65535, batch * seq below 2^31.  The _int8 form
  * returns h as codes q [batch * seq, dim] with scales s [batch * seq]. */
 int afb_sandwich_norm(const void* x, const void* residual, const void* gate,
                       const void* post_weight, const void* pre_weight, const void* shift,

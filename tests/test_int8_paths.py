@@ -58,3 +58,19 @@ def test_outputs_are_contiguous_whatever_the_inputs_are():
                 *ops.sandwich_norm_int8(x, x, None, w, w, None, None, 1.0, 1e-6),
                 *ops.sandwich_norm_bwd(x, None, x, x, None, w, w, None, 1.0, 1e-6))
         assert len(outs) == 24 and all(t.is_contiguous() for t in outs)
+
+
+def test_sizes_beyond_the_launches_are_refused():
+    """With a ValueError, like every other size, on fake CUDA tensors."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        e = lambda *s, d=torch.bfloat16: torch.empty(*s, dtype=d, device="cuda")  # noqa: E731
+        w = e(16, d=torch.float32)
+        for x in (e(65536, 1, 16), e(4, 2**29, 16)):
+            for call in (lambda: afb.sandwich_norm(x, x, None, w, w), lambda: afb.sandwich_norm_int8(x, x, None, w, w),
+                         lambda: afb.sandwich_norm_bwd(x, None, x, x, None, w, w)):
+                with pytest.raises(ValueError, match="65535"):
+                    call()
+        with pytest.raises(ValueError, match="2\\^20"):
+            afb.int8_wgrad(e(2, 2**20 + 8), e(2, 16, d=torch.int8), e(2, 1, d=torch.float32))
