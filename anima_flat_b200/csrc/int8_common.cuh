@@ -43,13 +43,12 @@ __device__ __forceinline__ float max_abs_nan(float m, f2_t v) {
 }
 // Maximum over the warp of bit patterns of non-negative floats: it orders
 // finite < infinity < NaN, so a row with a non-finite value keeps it.
+__device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(kFull, v); }
 // The group's maximum from its warps' in red[0 .. GROUP).
 template <int GROUP>
 __device__ __forceinline__ uint32_t group_max_u32(const uint32_t* red) {
-  const uint32_t v = red[(threadIdx.x & 31) % GROUP];
-  return __reduce_max_sync(kFull, v);
+  return warp_max_u32(red[(threadIdx.x & 31) % GROUP]);
 }
-__device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(kFull, v); }
 
 // Row quantisation.  With a = max(max|y|, 1e-30):
 //   s = a / 127,  q = rint(127 y / a), half to even.

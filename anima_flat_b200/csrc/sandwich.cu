@@ -452,9 +452,9 @@ struct SandwichBwdArgs {
 //
 // All six sums of a row are taken at once, with t = x gate post, since
 //   sum m xh = r1 (sum gz t + r2 (sum p t - r2 mean(p zh) sum z t)):
-// one barrier a pair of rows, and dx in the pass that forms dz (8192 x 2048: 44.9
-// us, 46.0 with a barrier of its own for sum m xh).  With the sums' kernel below
-// 43.5 us, 4096 x 2048 27.8, some 12 of which do not depend on the rows (launches,
+// one barrier a pair of rows, and dx in the pass that forms dz: 1.1 us less at
+// 8192 x 2048 than with a barrier of its own for sum m xh.  Both launches, with the
+// sums' kernel below: 8192 x 2048 43.5 us, 4096 x 2048 27.8, some 12 of which do not depend on the rows (launches,
 // first and last copies, the columns' sums).  In the row loop 16 warps fill 52%
 // of the issue slots, with 43 instructions an element; they wait for barriers and
 // shared memory in equal parts.
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kTeamThreads, 1) sandwich_bwd_kernel(const San
   for (int i = 0; i < mine; ++i) {
     const int r = (i * teams + team) * R;
     // A thread reads its own 16 bytes of each row alone; one past the last
-    // column reads column 0 and counts nothing.
+    // column reads nothing, and its sums are zero.
     uint8_t* at = dyn + (team * NS + i % NS) * stage_bytes + (col ? tid * 16 : 0);
     auto piece = [&](int k, int t) -> uint8_t* { return at + (k * 4 + t) * row_bytes; };
     ok = ok && mbar_wait(bar0 + 8 * (i % NS), (i / NS) & 1);

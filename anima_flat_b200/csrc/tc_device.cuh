@@ -1,5 +1,6 @@
 // Tensor-core building blocks: TMA tensor maps, tcgen05 matrix instructions
-// and tensor memory.  No cluster multicast is used.
+// and tensor memory.  No load is multicast; a pair's commit arrives on both its
+// CTAs' barriers.
 #pragma once
 
 #include <cuda.h>

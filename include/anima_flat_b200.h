@@ -270,8 +270,8 @@ int afb_rms_silu_bwd(const void* s, const void* gamma, const void* dy, const voi
 /* ----------------------------------------------------------------------- */
 /* 8-bit integer linear and 8-bit checkpoints (no reference counterpart)    */
 /* ----------------------------------------------------------------------- */
-/* dtype: type of the activations, 0 bf16 or 1 fp16.  Codes are int8; a row of
- * codes has one fp32 scale: with a = max(max|y|, 1e-30) over the row,
+/* dtype: type of the activations, 0 bf16 or 1 fp16.  Codes are int8 from -127 to
+ * 127; a row of codes has one fp32 scale: with a = max(max|y|, 1e-30) over the row,
  * s = a / 127 and q = rint(127 y / a), half to even.  A row that holds an
  * infinity or a NaN gets that as its scale and zero codes.  K a multiple of
  * 16, at most 16384 unless said otherwise; rows = 0 does nothing. */
